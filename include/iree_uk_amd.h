@@ -733,6 +733,212 @@ IREE_UK_AMD_EXPORT void iree_uk_amd_mmt4d_dequant_unpack_p(
     const iree_uk_amd_mmt4d_dequant_unpack_params_t* params);
 
 /*===----------------------------------------------------------------------===*/
+/* Between two products: row-wise steps into tiles, and a product's epilogue   */
+/*===----------------------------------------------------------------------===*/
+
+/* No counterpart in the reference, whose compiler generates these steps as
+ * dispatches of their own. A layer of a language model is then a short run of
+ * calls that hand each other tiles and row-major matrices:
+ *
+ *   iree_uk_amd_rmsnorm_pack            residual stream -> tiles
+ *   iree_uk_amd_mmt4d_epilogue_unpack   tiles x weights -> row-major matrix
+ *   iree_uk_amd_gate_pack               its halves (gate, up) -> tiles
+ *   iree_uk_amd_mmt4d_epilogue_unpack   tiles x weights + residual stream
+ *
+ * Flag values of the three calls; every call takes the groups it names. */
+enum {
+  /* Element type of the row-major inputs (the values of the pack types). */
+  IREE_UK_AMD_FLAG_IN_TYPE_MASK = 0x0F,
+  IREE_UK_AMD_FLAG_IN_TYPE_F32 = 0x01,
+  IREE_UK_AMD_FLAG_IN_TYPE_F16 = 0x04,
+  IREE_UK_AMD_FLAG_IN_TYPE_BF16 = 0x05,
+  /* Element type of the output. */
+  IREE_UK_AMD_FLAG_OUT_TYPE_MASK = 0xF0,
+  IREE_UK_AMD_FLAG_OUT_TYPE_F32 = 0x10,
+  IREE_UK_AMD_FLAG_OUT_TYPE_S8 = 0x20,
+  IREE_UK_AMD_FLAG_OUT_TYPE_F16 = 0x40,
+  IREE_UK_AMD_FLAG_OUT_TYPE_BF16 = 0x50,
+  IREE_UK_AMD_FLAG_OUT_TYPE_F8E4M3FN = 0x80,
+  /* Activation:  NONE  x;  RELU  x < 0 ? 0 : x;  SILU  x / (1 + e^-x);
+   *   GELU       x/2 * (1 + erf(x / sqrt 2));
+   *   GELU_TANH  x/2 * (1 + tanh(sqrt(2/pi) * (x + 0.044715 x^3))). */
+  IREE_UK_AMD_FLAG_ACTIVATION_MASK = 0xF00,
+  IREE_UK_AMD_FLAG_ACTIVATION_NONE = 0x000,
+  IREE_UK_AMD_FLAG_ACTIVATION_RELU = 0x100,
+  IREE_UK_AMD_FLAG_ACTIVATION_GELU = 0x200,
+  IREE_UK_AMD_FLAG_ACTIVATION_GELU_TANH = 0x300,
+  IREE_UK_AMD_FLAG_ACTIVATION_SILU = 0x400,
+};
+
+/* Root-mean-square norm of the rows of a row-major in_size0 x in_size1 matrix
+ * into tiles, with the residual's addition in front. Row by row, in f32:
+ *
+ *   h = in + residual                        (no residual_buffer: h = in)
+ *   sum = h                                  (rounded to the in type)
+ *   y = h / sqrt(mean(h^2) + epsilon) * weight     (no weight: 1)
+ *
+ * The norm is that of h before its rounding. y goes into out
+ * [out_size0][out_size1][out_size2][out_size3] = [M1][K1][M0][K0], the layout
+ * of iree_uk_pack without transposes and of an mmt4d left-hand side (M0 = 1:
+ * rows as they are), with zeros where the tiles reach beyond the matrix:
+ *   out type = in type   y, rounded;
+ *   S8, F8E4M3FN         y / row_scale[row], rounded to nearest even, with
+ *                        row_scale[row] = max|y| / 127 (S8), / 448 (F8E4M3FN):
+ *                        the row scales of iree_uk_amd_mmt4d_dequant_unpack
+ *                        and iree_uk_amd_mmt4d_epilogue_unpack.
+ * Rows with no 8-bit form: where max|y| is zero (or below 2^-100, whose scale
+ * has no usable inverse) the scale is 0 and the row zeros; where the row holds
+ * a NaN or an infinity, or its sum of squares exceeds f32, the scale is NaN and
+ * the row zeros, so that every result that the row enters is NaN.
+ *
+ * in, residual and sum have the in type, rows of contiguous columns and
+ * strides of their own, in elements, not negative; sum_buffer may be NULL (not
+ * asked for; only with a residual) and may be in_buffer or residual_buffer
+ * itself, with that one's offset and stride. weight: in_size1 entries of the in
+ * type, or NULL. row_scale: in_size0 entries, for the 8-bit types, else not
+ * used. out_stride0 >= 0, tile sizes as for iree_uk_pack; rows of sum and
+ * row_scale beyond in_size0 stay as they are. */
+typedef struct iree_uk_amd_rmsnorm_pack_params_t {
+  const void* in_buffer;
+  iree_uk_index_t in_offset;
+  iree_uk_index_t in_stride0;
+  const void* residual_buffer;
+  iree_uk_index_t residual_offset;
+  iree_uk_index_t residual_stride0;
+  void* sum_buffer;
+  iree_uk_index_t sum_offset;
+  iree_uk_index_t sum_stride0;
+  const void* weight;
+  float epsilon;
+  void* out_buffer;
+  iree_uk_index_t out_offset;
+  iree_uk_index_t out_stride0;
+  float* row_scale;
+  iree_uk_index_t in_size0;
+  iree_uk_index_t in_size1;
+  iree_uk_index_t out_size0;
+  iree_uk_index_t out_size1;
+  iree_uk_index_t out_size2;
+  iree_uk_index_t out_size3;
+  uint32_t flags; /* in type | out type */
+  const uint64_t* cpu_data;
+} iree_uk_amd_rmsnorm_pack_params_t;
+
+IREE_UK_AMD_EXPORT void iree_uk_amd_rmsnorm_pack(
+    const void* in_buffer, iree_uk_index_t in_offset,
+    iree_uk_index_t in_stride0, const void* residual_buffer,
+    iree_uk_index_t residual_offset, iree_uk_index_t residual_stride0,
+    void* sum_buffer, iree_uk_index_t sum_offset, iree_uk_index_t sum_stride0,
+    const void* weight, float epsilon, void* out_buffer,
+    iree_uk_index_t out_offset, iree_uk_index_t out_stride0, float* row_scale,
+    iree_uk_index_t in_size0, iree_uk_index_t in_size1,
+    iree_uk_index_t out_size0, iree_uk_index_t out_size1,
+    iree_uk_index_t out_size2, iree_uk_index_t out_size3, uint32_t flags,
+    const uint64_t* cpu_data);
+IREE_UK_AMD_EXPORT void iree_uk_amd_rmsnorm_pack_p(
+    const iree_uk_amd_rmsnorm_pack_params_t* params);
+
+/* An activation and the product with a second matrix, row-major into tiles:
+ *
+ *   y = activation(gate) * up                (no up_buffer: activation(gate))
+ *
+ * in f32, then as in iree_uk_amd_rmsnorm_pack: the same out types, row scales,
+ * rows without an 8-bit form, strides and tiles. gate and up are in_size0 x
+ * in_size1 and may be two halves of one matrix. Without an up_buffer and with
+ * ACTIVATION_NONE this is a pack that quantizes. */
+typedef struct iree_uk_amd_gate_pack_params_t {
+  const void* gate_buffer;
+  iree_uk_index_t gate_offset;
+  iree_uk_index_t gate_stride0;
+  const void* up_buffer;
+  iree_uk_index_t up_offset;
+  iree_uk_index_t up_stride0;
+  void* out_buffer;
+  iree_uk_index_t out_offset;
+  iree_uk_index_t out_stride0;
+  float* row_scale;
+  iree_uk_index_t in_size0;
+  iree_uk_index_t in_size1;
+  iree_uk_index_t out_size0;
+  iree_uk_index_t out_size1;
+  iree_uk_index_t out_size2;
+  iree_uk_index_t out_size3;
+  uint32_t flags; /* in type | out type | activation */
+  const uint64_t* cpu_data;
+} iree_uk_amd_gate_pack_params_t;
+
+IREE_UK_AMD_EXPORT void iree_uk_amd_gate_pack(
+    const void* gate_buffer, iree_uk_index_t gate_offset,
+    iree_uk_index_t gate_stride0, const void* up_buffer,
+    iree_uk_index_t up_offset, iree_uk_index_t up_stride0, void* out_buffer,
+    iree_uk_index_t out_offset, iree_uk_index_t out_stride0, float* row_scale,
+    iree_uk_index_t in_size0, iree_uk_index_t in_size1,
+    iree_uk_index_t out_size0, iree_uk_index_t out_size1,
+    iree_uk_index_t out_size2, iree_uk_index_t out_size3, uint32_t flags,
+    const uint64_t* cpu_data);
+IREE_UK_AMD_EXPORT void iree_uk_amd_gate_pack_p(
+    const iree_uk_amd_gate_pack_params_t* params);
+
+/* iree_uk_amd_mmt4d_dequant_unpack with the rest of a linear layer behind the
+ * scales: a row-major out_size0 x out_size1 matrix of f32, f16 or bf16 with
+ *
+ *   z[i][j] = (float)(sum_k lhs[i][k] * rhs[j][k]) * row_scale[i] * col_scale[j]
+ *   out[i][j] = residual[i][j] + activation(z[i][j] + bias[j])
+ *
+ * evaluated in f32 from left to right and rounded once, at the end. row_scale,
+ * bias, col_scale: out_size0 / out_size1 f32 entries; any of them may be NULL
+ * and then reads as 1, 0 and 1. residual_buffer: a matrix of the out type with
+ * a stride of its own, or NULL; it may be the output itself (same offset and
+ * stride), else the two do not overlap. Operand arguments, tile sizes and
+ * `flags` are those of iree_uk_mmt4d for a type with a 32-bit accumulator,
+ * without ACCUMULATE; `epilogue_flags` is out type | activation. K == 0 is a
+ * product of zeros. out_size0 <= M*M0 and out_size1 <= N*N0; elements between
+ * and behind the rows stay as they are. */
+typedef struct iree_uk_amd_mmt4d_epilogue_unpack_params_t {
+  const void* lhs_buffer;
+  iree_uk_index_t lhs_offset;
+  iree_uk_index_t lhs_stride0;
+  const void* rhs_buffer;
+  iree_uk_index_t rhs_offset;
+  iree_uk_index_t rhs_stride0;
+  const void* residual_buffer;
+  iree_uk_index_t residual_offset;
+  iree_uk_index_t residual_stride0;
+  void* out_buffer;
+  iree_uk_index_t out_offset;
+  iree_uk_index_t out_stride0;
+  iree_uk_index_t out_size0;
+  iree_uk_index_t out_size1;
+  const float* row_scale;
+  const float* col_scale;
+  const float* bias;
+  iree_uk_index_t M;
+  iree_uk_index_t N;
+  iree_uk_index_t K;
+  int32_t M0;
+  int32_t N0;
+  int32_t K0;
+  uint32_t flags;
+  uint32_t epilogue_flags;
+  const uint64_t* cpu_data;
+} iree_uk_amd_mmt4d_epilogue_unpack_params_t;
+
+IREE_UK_AMD_EXPORT void iree_uk_amd_mmt4d_epilogue_unpack(
+    const void* lhs_buffer, iree_uk_index_t lhs_offset,
+    iree_uk_index_t lhs_stride0, const void* rhs_buffer,
+    iree_uk_index_t rhs_offset, iree_uk_index_t rhs_stride0,
+    const void* residual_buffer, iree_uk_index_t residual_offset,
+    iree_uk_index_t residual_stride0, void* out_buffer,
+    iree_uk_index_t out_offset, iree_uk_index_t out_stride0,
+    iree_uk_index_t out_size0, iree_uk_index_t out_size1,
+    const float* row_scale, const float* col_scale, const float* bias,
+    iree_uk_index_t M, iree_uk_index_t N, iree_uk_index_t K, int32_t M0,
+    int32_t N0, int32_t K0, uint32_t flags, uint32_t epilogue_flags,
+    const uint64_t* cpu_data);
+IREE_UK_AMD_EXPORT void iree_uk_amd_mmt4d_epilogue_unpack_p(
+    const iree_uk_amd_mmt4d_epilogue_unpack_params_t* params);
+
+/*===----------------------------------------------------------------------===*/
 /* HAL executable plugin face                                                  */
 /*===----------------------------------------------------------------------===*/
 

@@ -47,6 +47,10 @@ extern "C" int iree_uk_amd_hip_launch_mmt4d(const iree_uk_mmt4d_params_t* p,
   // Every call starts from "one K slice": the barrier-free matrix-core kernels and the
   // 128x128 blocks in slices report more (iree_uk_amd_last_k_slices).
   uk_mfma::note_k_slices(1);
+  if (rowmajor && rowmajor->epilogue) {
+    *kernel_name = "mmt4d_generic";
+    return iree_uk_amd_hip_launch_mmt4d_generic(p, rowmajor, stream);
+  }
   // s8 x s4 -> s32 and s16 x s16 -> s32 have an MFMA kernel for some shapes
   // only; the launcher says "not served" (negative) for the rest.
   const uint32_t type = p->flags & IREE_UK_FLAG_MMT4D_TYPE_MASK;

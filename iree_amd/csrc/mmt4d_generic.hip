@@ -7,6 +7,7 @@
 // round after the multiply and after the add, like the CPU build.
 #include <hip/hip_runtime.h>
 
+#include "uk_activation.h"
 #include "uk_device_common.h"
 #include "uk_float_convert.h"
 #include "uk_hip_abi.h"
@@ -54,6 +55,11 @@ struct Mmt4dArgs {
   int64_t acc_s_i;
   const float* row_scale;
   const float* col_scale;
+  // The rest of a linear layer behind the dequantizing store (iree_uk_amd_rowmajor_out_t).
+  uint32_t epilogue, out_type, act;
+  const float* bias;
+  const char* residual;
+  int64_t residual_stride;  // elements
   int64_t M, N, K;
   int32_t M0, N0, K0;
   uint32_t accumulate, skip_round;
@@ -87,6 +93,26 @@ __global__ __launch_bounds__(kThreads) void mmt4d_generic_kernel(Mmt4dArgs a) {
       const float cs = a.col_scale ? a.col_scale[j * N0 + j0] : 1.0f;
       return v * rs * cs;
     };
+    // The dequantizing store, with what follows the scales of a linear layer.
+    auto store_scaled = [&](float acc) {
+      float v = scaled(acc);
+      if (!a.epilogue) {
+        reinterpret_cast<float*>(a.out)[o] = v;
+        return;
+      }
+      if (a.bias) v += a.bias[j * N0 + j0];
+      v = uk::activate(v, a.act);
+      const int64_t ro = (i * M0 + i0) * a.residual_stride + j * N0 + j0;
+      auto store = [&](auto type) {
+        using F = decltype(type);
+        using T = typename F::T;
+        if (a.residual) v = F::to_f32(reinterpret_cast<const T*>(a.residual)[ro]) + v;
+        reinterpret_cast<T*>(a.out)[o] = F::from_f32(v);
+      };
+      if (a.out_type == IREE_UK_AMD_FLAG_OUT_TYPE_F32) store(uk::F32{});
+      else if (a.out_type == IREE_UK_AMD_FLAG_OUT_TYPE_F16) store(uk::F16{});
+      else store(uk::BF16{});
+    };
 
     if constexpr (KIND == Kind::kS8S8 || KIND == Kind::kS16S16 || KIND == Kind::kS16S8) {
       int32_t* out = reinterpret_cast<int32_t*>(a.out);
@@ -103,7 +129,7 @@ __global__ __launch_bounds__(kThreads) void mmt4d_generic_kernel(Mmt4dArgs a) {
           acc += (uint32_t)(l * r);
         }
       }
-      if (a.dequant) reinterpret_cast<float*>(a.out)[o] = scaled((float)(int32_t)acc);
+      if (a.dequant) store_scaled((float)(int32_t)acc);
       else out[o] = (int32_t)acc;
     } else if constexpr (KIND == Kind::kS8S4 || KIND == Kind::kS16U4) {
       // Two 4-bit rhs values per byte, low nibble first.
@@ -131,7 +157,7 @@ __global__ __launch_bounds__(kThreads) void mmt4d_generic_kernel(Mmt4dArgs a) {
           acc += (uint32_t)(l0 * r0 + l1 * r1);
         }
       }
-      if (a.dequant) reinterpret_cast<float*>(a.out)[o] = scaled((float)(int32_t)acc);
+      if (a.dequant) store_scaled((float)(int32_t)acc);
       else out[o] = (int32_t)acc;
     } else if constexpr (KIND == Kind::kF32 || KIND == Kind::kF16F32 ||
                          KIND == Kind::kBF16F32 || KIND == Kind::kF8F32) {
@@ -158,7 +184,8 @@ __global__ __launch_bounds__(kThreads) void mmt4d_generic_kernel(Mmt4dArgs a) {
           acc += l * r;
         }
       }
-      out[o] = a.dequant ? scaled(acc) : acc;
+      if (a.dequant) store_scaled(acc);
+      else out[o] = acc;
     } else {
       // f16 / bf16 results, with or without rounding the running sum to the
       // 16-bit type after every multiply-add.
@@ -239,6 +266,18 @@ extern "C" int iree_uk_amd_hip_launch_mmt4d_generic(
     a.acc_s_i = rowmajor->acc_stride0;
     a.row_scale = rowmajor->row_scale;
     a.col_scale = rowmajor->col_scale;
+  }
+  a.epilogue = rowmajor && rowmajor->epilogue;
+  a.out_type = a.act = 0;
+  a.bias = nullptr;
+  a.residual = nullptr;
+  a.residual_stride = 0;
+  if (a.epilogue) {
+    a.out_type = rowmajor->epilogue_flags & IREE_UK_AMD_FLAG_OUT_TYPE_MASK;
+    a.act = rowmajor->epilogue_flags & IREE_UK_AMD_FLAG_ACTIVATION_MASK;
+    a.bias = rowmajor->bias;
+    a.residual = (const char*)rowmajor->residual;
+    a.residual_stride = rowmajor->residual_stride0;
   }
   a.M = p->M; a.N = p->N; a.K = p->K;
   a.M0 = p->M0; a.N0 = p->N0; a.K0 = p->K0;

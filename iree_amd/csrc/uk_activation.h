@@ -1,0 +1,73 @@
+// Activations and float conversions of the row-wise steps and of the products'
+// epilogue. Device code.
+#ifndef IREE_UK_AMD_ACTIVATION_H_
+#define IREE_UK_AMD_ACTIVATION_H_
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "iree_uk_amd.h"
+
+namespace uk {
+
+// x * sigmoid(t) = x / (1 + 2^(-t log2 e)). An exponent of 128 and more gives an
+// infinity, and x over it zero, which is what the product tends to (from 2^126 on already:
+// the reciprocal would be subnormal, and the hardware's is zero). The hardware's
+// exponential and reciprocal are good to one unit in the last place each: the
+// result to about three, and to |t| units where t is large and negative.
+__device__ __forceinline__ float times_sigmoid(float x, float t) {
+  return x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504f * t));
+}
+
+// x Phi(x) with Phi(x) = erfc(-x / sqrt 2) / 2, by the approximation of Hastings that
+// Abramowitz and Stegun give as 7.1.26 (erfc(z) = e^(-z^2) p(t), t = 1 / (1 + 0.3275911 z),
+// to 1.5e-7 for z >= 0): x - x erfc(z) / 2 for positive x, x erfc(z) / 2 for negative,
+// so nothing cancels in the negative tail.
+__device__ __forceinline__ float gelu(float x) {
+  const float ax = __builtin_fabsf(x);
+  const float z = ax * 0.70710678f;
+  const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f, z, 1.0f));
+  float p = __builtin_fmaf(1.061405429f, t, -1.453152027f);
+  p = __builtin_fmaf(p, t, 1.421413741f);
+  p = __builtin_fmaf(p, t, -0.284496736f);
+  p = __builtin_fmaf(p, t, 0.254829592f);
+  // (An infinite x has a tail of infinity times zero; its limit is zero.)
+  const float e = __builtin_amdgcn_exp2f(-1.44269504f * z * z);
+  const float tail = e == 0.0f ? 0.0f : 0.5f * ax * (p * t * e);
+  return x > 0.0f ? x - tail : x < 0.0f ? -tail : x;
+}
+
+// `act` is an IREE_UK_AMD_FLAG_ACTIVATION_* value, the same in all lanes. The comparison of
+// RELU lets a NaN through.
+__device__ __forceinline__ float activate(float x, uint32_t act) {
+  switch (act) {
+    case IREE_UK_AMD_FLAG_ACTIVATION_RELU: return x < 0.0f ? 0.0f : x;
+    case IREE_UK_AMD_FLAG_ACTIVATION_GELU: return gelu(x);
+    // tanh(u) = 2 sigmoid(2 u) - 1, so x / 2 * (1 + tanh(u)) = x sigmoid(2 u).
+    case IREE_UK_AMD_FLAG_ACTIVATION_GELU_TANH:
+      return times_sigmoid(x, x * __builtin_fmaf(0.0713548163f, x * x, 1.59576912f));
+    case IREE_UK_AMD_FLAG_ACTIVATION_SILU: return times_sigmoid(x, x);
+    default: return x;
+  }
+}
+
+// f32 to and from the 16-bit floats, rounded to nearest even, subnormals kept.
+struct F32 {
+  typedef float T;
+  static __device__ __forceinline__ float to_f32(T v) { return v; }
+  static __device__ __forceinline__ T from_f32(float v) { return v; }
+};
+struct F16 {
+  typedef _Float16 T;
+  static __device__ __forceinline__ float to_f32(T v) { return (float)v; }
+  static __device__ __forceinline__ T from_f32(float v) { return (_Float16)v; }
+};
+struct BF16 {
+  typedef __bf16 T;
+  static __device__ __forceinline__ float to_f32(T v) { return (float)v; }
+  static __device__ __forceinline__ T from_f32(float v) { return (__bf16)v; }
+};
+
+}  // namespace uk
+
+#endif  // IREE_UK_AMD_ACTIVATION_H_

@@ -43,6 +43,17 @@ typedef struct iree_uk_amd_rowmajor_out_t {
   const float* col_scale;
   const void* acc;
   int64_t acc_stride0;
+  /* The rest of a linear layer behind the dequantizing store
+   * (iree_uk_amd_mmt4d_epilogue_unpack); `epilogue` 0: none and the fields below
+   * are not read. The matrix has the out type of `epilogue_flags`, its address
+   * is the params' out_buffer (out_offset 0); element (i, j) is residual[i][j]
+   * + activation(z + bias[j]) with z as above. `residual`: first element, or
+   * NULL; `residual_stride0` elements between its rows. */
+  int epilogue;
+  uint32_t epilogue_flags;
+  const float* bias;
+  const void* residual;
+  int64_t residual_stride0;
 } iree_uk_amd_rowmajor_out_t;
 
 /* `rowmajor` NULL: the result is stored tiled, as iree_uk_mmt4d does. */
@@ -50,6 +61,28 @@ int iree_uk_amd_hip_launch_mmt4d(const iree_uk_mmt4d_params_t* params,
                                  const iree_uk_amd_rowmajor_out_t* rowmajor,
                                  void* stream, int kernel_mode,
                                  const char** kernel_name);
+
+/* The row-wise steps into tiles (iree_uk_amd_rmsnorm_pack, iree_uk_amd_gate_pack).
+ * Addresses are those of first elements, strides in elements. */
+typedef struct iree_uk_amd_row_op_t {
+  int norm; /* 1: rmsnorm_pack, 0: gate_pack */
+  const void* in;
+  int64_t in_stride0;
+  const void* second; /* residual or up, may be NULL */
+  int64_t second_stride0;
+  void* sum; /* norm only, may be NULL */
+  int64_t sum_stride0;
+  const void* weight; /* norm only, may be NULL */
+  float epsilon;      /* norm only */
+  void* out;
+  int64_t out_stride0;
+  float* row_scale; /* 8-bit out types */
+  int64_t rows, cols;
+  int64_t M1, K1, M0, K0;
+  uint32_t flags;
+} iree_uk_amd_row_op_t;
+int iree_uk_amd_hip_launch_row_op(const iree_uk_amd_row_op_t* op, void* stream,
+                                  const char** kernel_name);
 
 int iree_uk_amd_hip_launch_conv_nchwc(const iree_uk_conv_nchwc_params_t* params,
                                       void* stream, int kernel_mode,

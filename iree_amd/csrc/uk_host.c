@@ -110,6 +110,31 @@ static int mmt4d_type_bits(uint32_t flags, mmt4d_bits_t* b) {
   }
 }
 
+static uint32_t in_type(uint32_t flags) {
+  return flags & IREE_UK_AMD_FLAG_IN_TYPE_MASK;
+}
+static uint32_t out_type(uint32_t flags) {
+  return flags & IREE_UK_AMD_FLAG_OUT_TYPE_MASK;
+}
+
+/* Bytes of an element of an in type or an out type; 0 for an unknown one. */
+static int float_type_bytes(uint32_t type) {
+  switch (type) {
+    case IREE_UK_AMD_FLAG_IN_TYPE_F32:
+    case IREE_UK_AMD_FLAG_OUT_TYPE_F32: return 4;
+    case IREE_UK_AMD_FLAG_IN_TYPE_F16:
+    case IREE_UK_AMD_FLAG_IN_TYPE_BF16:
+    case IREE_UK_AMD_FLAG_OUT_TYPE_F16:
+    case IREE_UK_AMD_FLAG_OUT_TYPE_BF16: return 2;
+    default: return 0;
+  }
+}
+
+static int is_8bit_type(uint32_t type) {
+  return type == IREE_UK_AMD_FLAG_OUT_TYPE_S8 ||
+         type == IREE_UK_AMD_FLAG_OUT_TYPE_F8E4M3FN;
+}
+
 /* pack and unpack share type values; unpack has no 1-byte type
  * (exported_bits.h:56-62,73-79). */
 static int pack_elem_bytes(uint32_t flags) {
@@ -352,7 +377,10 @@ static void mmt4d_run(const iree_uk_mmt4d_params_t* params,
   iree_uk_amd_rowmajor_out_t rm;
   if (rowmajor) rm = *rowmajor;
   else memset(&rm, 0, sizeof rm);
-  const int out_bytes = bits.out_bits / 8;
+  const int epilogue = rowmajor && rm.epilogue;
+  const int acc_bytes = bits.out_bits / 8;
+  const int out_bytes =
+      epilogue ? float_type_bytes(out_type(rm.epilogue_flags)) : acc_bytes;
   staged_t lhs = staged((char*)p.lhs_buffer + p.lhs_offset * bits.lhs_bits / 8,
                   p.lhs_stride0 * bits.lhs_bits / 8,
                   p.K * p.M0 * p.K0 * bits.lhs_bits / 8, p.M);
@@ -371,12 +399,13 @@ static void mmt4d_run(const iree_uk_mmt4d_params_t* params,
    * initial accumulators (ACCUMULATE) come from a tiled buffer of their own. */
   const int dequant = rowmajor && rm.dequant;
   const int accumulate = (p.flags & IREE_UK_FLAG_MMT4D_ACCUMULATE) != 0;
-  staged_t acc = staged(0, 0, 0, 0), rscale = acc, cscale = acc;
+  staged_t acc = staged(0, 0, 0, 0), rscale = acc, cscale = acc, bias = acc,
+           residual = acc;
   if (dequant) {
     if (accumulate) {
       acc.host_base = (char*)rm.acc;
-      acc.pitch = rm.acc_stride0 * out_bytes;
-      acc.row_bytes = p.N * p.M0 * p.N0 * out_bytes;
+      acc.pitch = rm.acc_stride0 * acc_bytes;
+      acc.row_bytes = p.N * p.M0 * p.N0 * acc_bytes;
       acc.rows = p.M;
     }
     if (rm.row_scale) {
@@ -390,13 +419,32 @@ static void mmt4d_run(const iree_uk_mmt4d_params_t* params,
       cscale.rows = 1;
     }
   }
-  staged_t* ops[6] = {&lhs, &rhs, &out, &acc, &rscale, &cscale};
-  const int copy_in[6] = {1, 1, accumulate && !dequant, 1, 1, 1};
-  int st = stage_in(ops, copy_in, 6);
+  if (epilogue) {
+    if (rm.bias) {
+      bias.host_base = (char*)rm.bias;
+      bias.pitch = bias.row_bytes = rm.size1 * (int64_t)sizeof(float);
+      bias.rows = 1;
+    }
+    if (rm.residual) {
+      residual.host_base = (char*)rm.residual;
+      residual.pitch = rm.residual_stride0 * out_bytes;
+      residual.row_bytes = rm.size1 * out_bytes;
+      residual.rows = rm.size0;
+    }
+  }
+  staged_t* ops[8] = {&lhs,    &rhs,    &out,  &acc,
+                      &rscale, &cscale, &bias, &residual};
+  const int copy_in[8] = {1, 1, accumulate && !dequant, 1, 1, 1, 1, 1};
+  int st = stage_in(ops, copy_in, 8);
   if (!st) {
     if (acc.device) {
       rm.acc = acc.device;
-      rm.acc_stride0 = acc.device_pitch / out_bytes;
+      rm.acc_stride0 = acc.device_pitch / acc_bytes;
+    }
+    if (bias.device) rm.bias = (const float*)bias.device;
+    if (residual.device) {
+      rm.residual = residual.device;
+      rm.residual_stride0 = residual.device_pitch / out_bytes;
     }
     if (rscale.device) rm.row_scale = (const float*)rscale.device;
     if (cscale.device) rm.col_scale = (const float*)cscale.device;
@@ -420,7 +468,7 @@ static void mmt4d_run(const iree_uk_mmt4d_params_t* params,
                                       tls_kernel_mode, &tls_kernel_name);
   }
   if (!st) st = stage_out(&out);
-  st = stage_finish(st, ops, 6);
+  st = stage_finish(st, ops, 8);
   tls_status = st;
 }
 
@@ -580,6 +628,81 @@ void iree_uk_amd_mmt4d_dequant_unpack(
   iree_uk_amd_mmt4d_dequant_unpack_p(&params);
 }
 
+/* Fused mmt4d + epilogue: as for the dequantizing store, with a float matrix
+ * and nothing to accumulate onto. */
+static int mmt4d_epilogue_validate(
+    const iree_uk_amd_mmt4d_epilogue_unpack_params_t* p,
+    const iree_uk_mmt4d_params_t* mm) {
+  if (!mmt4d_validate(mm)) return 0;
+  mmt4d_bits_t bits;
+  mmt4d_type_bits(mm->flags, &bits);
+  UK_REQUIRE(bits.out_bits == 32);
+  UK_REQUIRE(!(p->flags & IREE_UK_FLAG_MMT4D_ACCUMULATE));
+  UK_REQUIRE(!(p->epilogue_flags & ~(uint32_t)(IREE_UK_AMD_FLAG_OUT_TYPE_MASK |
+                                               IREE_UK_AMD_FLAG_ACTIVATION_MASK)));
+  UK_REQUIRE(float_type_bytes(out_type(p->epilogue_flags)) != 0);
+  UK_REQUIRE((p->epilogue_flags & IREE_UK_AMD_FLAG_ACTIVATION_MASK) <=
+             IREE_UK_AMD_FLAG_ACTIVATION_SILU);
+  UK_REQUIRE(p->out_size0 >= 0 && p->out_size0 <= p->M * p->M0);
+  UK_REQUIRE(p->out_size1 >= 0 && p->out_size1 <= p->N * p->N0);
+  UK_REQUIRE(p->out_stride0 >= 0 && p->residual_stride0 >= 0);
+  return 1;
+}
+
+void iree_uk_amd_mmt4d_epilogue_unpack_p(
+    const iree_uk_amd_mmt4d_epilogue_unpack_params_t* params) {
+  tls_status = 0;
+  tls_kernel_name = "";
+  iree_uk_mmt4d_params_t mm = {
+      params->lhs_buffer, params->lhs_offset, params->lhs_stride0,
+      params->rhs_buffer, params->rhs_offset, params->rhs_stride0,
+      params->out_buffer, /*out_offset=*/0, /*out_stride0=*/0,
+      params->M, params->N, params->K, params->M0, params->N0, params->K0,
+      params->flags, params->cpu_data};
+  if (!mmt4d_epilogue_validate(params, &mm)) return;
+  /* Nothing to write. K == 0 writes what the epilogue makes of zeros. */
+  if (params->M == 0 || params->N == 0 || params->out_size0 == 0 ||
+      params->out_size1 == 0) {
+    return;
+  }
+  const int es = float_type_bytes(out_type(params->epilogue_flags));
+  mm.out_buffer = (char*)params->out_buffer + params->out_offset * es;
+  iree_uk_amd_rowmajor_out_t rm;
+  memset(&rm, 0, sizeof rm);
+  rm.stride0 = params->out_stride0;
+  rm.size0 = params->out_size0;
+  rm.size1 = params->out_size1;
+  rm.dequant = 1;
+  rm.row_scale = params->row_scale;
+  rm.col_scale = params->col_scale;
+  rm.epilogue = 1;
+  rm.epilogue_flags = params->epilogue_flags;
+  rm.bias = params->bias;
+  if (params->residual_buffer) {
+    rm.residual =
+        (const char*)params->residual_buffer + params->residual_offset * es;
+    rm.residual_stride0 = params->residual_stride0;
+  }
+  mmt4d_run(&mm, &rm);
+}
+
+void iree_uk_amd_mmt4d_epilogue_unpack(
+    const void* lhs_buffer, iree_uk_index_t lhs_offset, iree_uk_index_t lhs_stride0,
+    const void* rhs_buffer, iree_uk_index_t rhs_offset, iree_uk_index_t rhs_stride0,
+    const void* residual_buffer, iree_uk_index_t residual_offset,
+    iree_uk_index_t residual_stride0, void* out_buffer, iree_uk_index_t out_offset,
+    iree_uk_index_t out_stride0, iree_uk_index_t out_size0, iree_uk_index_t out_size1,
+    const float* row_scale, const float* col_scale, const float* bias, iree_uk_index_t M,
+    iree_uk_index_t N, iree_uk_index_t K, int32_t M0, int32_t N0, int32_t K0,
+    uint32_t flags, uint32_t epilogue_flags, const uint64_t* cpu_data) {
+  iree_uk_amd_mmt4d_epilogue_unpack_params_t params = {
+      lhs_buffer, lhs_offset, lhs_stride0, rhs_buffer, rhs_offset, rhs_stride0,
+      residual_buffer, residual_offset, residual_stride0, out_buffer, out_offset,
+      out_stride0, out_size0, out_size1, row_scale, col_scale, bias, M, N, K,
+      M0, N0, K0, flags, epilogue_flags, cpu_data};
+  iree_uk_amd_mmt4d_epilogue_unpack_p(&params);
+}
+
 void iree_uk_mmt4d(const void* lhs_buffer, iree_uk_index_t lhs_offset,
                    iree_uk_index_t lhs_stride0, const void* rhs_buffer,
                    iree_uk_index_t rhs_offset, iree_uk_index_t rhs_stride0,
@@ -688,6 +811,173 @@ void iree_uk_pack(const void* in_buffer, iree_uk_index_t in_offset,
       out_stride0, out_stride1, in_size0, in_size1, out_size0,     out_size1,
       out_size2, out_size3, padding_value, flags,   cpu_data};
   iree_uk_pack_p(&params);
+}
+
+/*---------------------------------------------------------------------------
+ * Row-wise steps into tiles
+ *-------------------------------------------------------------------------*/
+
+/* What both calls ask of types, sizes and strides; tiles as pack_validate. */
+static int row_op_validate(const iree_uk_amd_row_op_t* p) {
+  UK_REQUIRE(!(p->flags & ~(uint32_t)(IREE_UK_AMD_FLAG_IN_TYPE_MASK |
+                                      IREE_UK_AMD_FLAG_OUT_TYPE_MASK |
+                                      IREE_UK_AMD_FLAG_ACTIVATION_MASK)));
+  const uint32_t in = in_type(p->flags), out = out_type(p->flags);
+  UK_REQUIRE(in != 0 && float_type_bytes(in) != 0);
+  UK_REQUIRE(out == in << 4 || is_8bit_type(out));
+  UK_REQUIRE((p->flags & IREE_UK_AMD_FLAG_ACTIVATION_MASK) <=
+             (p->norm ? IREE_UK_AMD_FLAG_ACTIVATION_NONE
+                      : IREE_UK_AMD_FLAG_ACTIVATION_SILU));
+  UK_REQUIRE(fits_unsigned_bits(p->rows, 31));
+  UK_REQUIRE(fits_unsigned_bits(p->cols, 31));
+  UK_REQUIRE(fits_unsigned_bits(p->M1, 31));
+  UK_REQUIRE(fits_unsigned_bits(p->K1, 31));
+  UK_REQUIRE(fits_unsigned_bits(p->M0, 15));
+  UK_REQUIRE(fits_unsigned_bits(p->K0, 15));
+  UK_REQUIRE(fits_unsigned_bits(p->M1 * p->M0, 31));
+  UK_REQUIRE(fits_unsigned_bits(p->K1 * p->K0, 31));
+  UK_REQUIRE(p->M1 * p->M0 >= p->rows);
+  UK_REQUIRE(p->K1 * p->K0 >= p->cols);
+  const int es = is_8bit_type(out) ? 1 : float_type_bytes(out);
+  UK_REQUIRE(p->M0 * p->K0 == 0 || ceil_pow2(p->M0 * p->K0 * es) <= 4096);
+  UK_REQUIRE(p->in_stride0 >= 0 && p->second_stride0 >= 0);
+  UK_REQUIRE(p->sum_stride0 >= 0 && p->out_stride0 >= 0);
+  UK_REQUIRE(!is_8bit_type(out) || p->rows == 0 || p->row_scale != 0);
+  UK_REQUIRE(!p->sum || p->second);
+  UK_REQUIRE(!p->norm || p->epsilon >= 0.0f);
+  return 1;
+}
+
+/* Runs a call whose addresses have their offsets applied. */
+static void row_op_run(iree_uk_amd_row_op_t p) {
+  if (!row_op_validate(&p)) return;
+  if (p.M1 == 0 || p.M0 == 0) return;
+  const int es = float_type_bytes(in_type(p.flags));
+  const int os = is_8bit_type(out_type(p.flags)) ? 1 : es;
+  staged_t in = staged(p.in, p.in_stride0 * es, p.cols * es, p.rows);
+  staged_t second = staged(p.second, p.second_stride0 * es, p.cols * es,
+                           p.second ? p.rows : 0);
+  staged_t sum =
+      staged(p.sum, p.sum_stride0 * es, p.cols * es, p.sum ? p.rows : 0);
+  staged_t weight = staged(p.weight, p.cols * es, p.cols * es, p.weight ? 1 : 0);
+  staged_t out = staged(p.out, p.out_stride0 * os, p.K1 * p.M0 * p.K0 * os, p.M1);
+  staged_t scale = staged(p.row_scale, p.rows * 4, p.rows * 4, os == 1 ? 1 : 0);
+  staged_t* ops[6] = {&in, &second, &sum, &weight, &out, &scale};
+  const int copy_in[6] = {1, 1, 0, 1, 0, 0}; /* outputs are written in full */
+  int st = stage_in(ops, copy_in, 6);
+  if (!st) {
+    if (in.device) {
+      p.in = in.device;
+      p.in_stride0 = in.device_pitch / es;
+    }
+    if (second.device) {
+      p.second = second.device;
+      p.second_stride0 = second.device_pitch / es;
+    }
+    if (sum.device) {
+      p.sum = sum.device;
+      p.sum_stride0 = sum.device_pitch / es;
+    }
+    if (weight.device) p.weight = weight.device;
+    if (out.device) {
+      p.out = out.device;
+      p.out_stride0 = out.device_pitch / os;
+    }
+    if (scale.device) p.row_scale = (float*)scale.device;
+    st = iree_uk_amd_hip_launch_row_op(&p, tls_stream, &tls_kernel_name);
+  }
+  if (!st) st = stage_out(&sum);
+  if (!st) st = stage_out(&out);
+  if (!st) st = stage_out(&scale);
+  st = stage_finish(st, ops, 6);
+  tls_status = st;
+}
+
+/* First element of a buffer, NULL for a buffer that is not there. */
+static void* at_element(const void* buffer, int64_t offset, int bytes) {
+  return buffer ? (char*)buffer + offset * bytes : 0;
+}
+
+void iree_uk_amd_rmsnorm_pack_p(const iree_uk_amd_rmsnorm_pack_params_t* params) {
+  tls_status = 0;
+  tls_kernel_name = "";
+  const int es = float_type_bytes(in_type(params->flags));
+  const int os = is_8bit_type(out_type(params->flags)) ? 1 : es;
+  const iree_uk_amd_row_op_t p = {
+      .norm = 1,
+      .in = at_element(params->in_buffer, params->in_offset, es),
+      .in_stride0 = params->in_stride0,
+      .second = at_element(params->residual_buffer, params->residual_offset, es),
+      .second_stride0 = params->residual_stride0,
+      .sum = at_element(params->sum_buffer, params->sum_offset, es),
+      .sum_stride0 = params->sum_stride0,
+      .weight = params->weight,
+      .epsilon = params->epsilon,
+      .out = at_element(params->out_buffer, params->out_offset, os),
+      .out_stride0 = params->out_stride0,
+      .row_scale = params->row_scale,
+      .rows = params->in_size0,
+      .cols = params->in_size1,
+      .M1 = params->out_size0,
+      .K1 = params->out_size1,
+      .M0 = params->out_size2,
+      .K0 = params->out_size3,
+      .flags = params->flags};
+  row_op_run(p);
+}
+
+void iree_uk_amd_rmsnorm_pack(
+    const void* in_buffer, iree_uk_index_t in_offset, iree_uk_index_t in_stride0,
+    const void* residual_buffer, iree_uk_index_t residual_offset,
+    iree_uk_index_t residual_stride0, void* sum_buffer, iree_uk_index_t sum_offset,
+    iree_uk_index_t sum_stride0, const void* weight, float epsilon, void* out_buffer,
+    iree_uk_index_t out_offset, iree_uk_index_t out_stride0, float* row_scale,
+    iree_uk_index_t in_size0, iree_uk_index_t in_size1, iree_uk_index_t out_size0,
+    iree_uk_index_t out_size1, iree_uk_index_t out_size2, iree_uk_index_t out_size3,
+    uint32_t flags, const uint64_t* cpu_data) {
+  iree_uk_amd_rmsnorm_pack_params_t params = {
+      in_buffer, in_offset, in_stride0, residual_buffer, residual_offset,
+      residual_stride0, sum_buffer, sum_offset, sum_stride0, weight, epsilon,
+      out_buffer, out_offset, out_stride0, row_scale, in_size0, in_size1,
+      out_size0, out_size1, out_size2, out_size3, flags, cpu_data};
+  iree_uk_amd_rmsnorm_pack_p(&params);
+}
+
+void iree_uk_amd_gate_pack_p(const iree_uk_amd_gate_pack_params_t* params) {
+  tls_status = 0;
+  tls_kernel_name = "";
+  const int es = float_type_bytes(in_type(params->flags));
+  const int os = is_8bit_type(out_type(params->flags)) ? 1 : es;
+  const iree_uk_amd_row_op_t p = {
+      .in = at_element(params->gate_buffer, params->gate_offset, es),
+      .in_stride0 = params->gate_stride0,
+      .second = at_element(params->up_buffer, params->up_offset, es),
+      .second_stride0 = params->up_stride0,
+      .out = at_element(params->out_buffer, params->out_offset, os),
+      .out_stride0 = params->out_stride0,
+      .row_scale = params->row_scale,
+      .rows = params->in_size0,
+      .cols = params->in_size1,
+      .M1 = params->out_size0,
+      .K1 = params->out_size1,
+      .M0 = params->out_size2,
+      .K0 = params->out_size3,
+      .flags = params->flags};
+  row_op_run(p);
+}
+
+void iree_uk_amd_gate_pack(
+    const void* gate_buffer, iree_uk_index_t gate_offset, iree_uk_index_t gate_stride0,
+    const void* up_buffer, iree_uk_index_t up_offset, iree_uk_index_t up_stride0,
+    void* out_buffer, iree_uk_index_t out_offset, iree_uk_index_t out_stride0,
+    float* row_scale, iree_uk_index_t in_size0, iree_uk_index_t in_size1,
+    iree_uk_index_t out_size0, iree_uk_index_t out_size1, iree_uk_index_t out_size2,
+    iree_uk_index_t out_size3, uint32_t flags, const uint64_t* cpu_data) {
+  iree_uk_amd_gate_pack_params_t params = {
+      gate_buffer, gate_offset, gate_stride0, up_buffer, up_offset, up_stride0,
+      out_buffer, out_offset, out_stride0, row_scale, in_size0, in_size1,
+      out_size0, out_size1, out_size2, out_size3, flags, cpu_data};
+  iree_uk_amd_gate_pack_p(&params);
 }
 
 /*---------------------------------------------------------------------------

@@ -49,6 +49,21 @@ UNPACK_TYPE_BF16BF16 = 0x05
 UNPACK_TRANSPOSE_INNER = 0x100
 UNPACK_TRANSPOSE_OUTER = 0x200
 
+# rmsnorm_pack, gate_pack and mmt4d_epilogue_unpack (extensions of this library)
+IN_TYPE_F32 = 0x01
+IN_TYPE_F16 = 0x04
+IN_TYPE_BF16 = 0x05
+OUT_TYPE_F32 = 0x10
+OUT_TYPE_S8 = 0x20
+OUT_TYPE_F16 = 0x40
+OUT_TYPE_BF16 = 0x50
+OUT_TYPE_F8E4M3FN = 0x80
+ACTIVATION_NONE = 0x000
+ACTIVATION_RELU = 0x100
+ACTIVATION_GELU = 0x200
+ACTIVATION_GELU_TANH = 0x300
+ACTIVATION_SILU = 0x400
+
 POINTER_MODE_AUTO = 0
 POINTER_MODE_DEVICE = 1
 KERNEL_MODE_AUTO = 0
@@ -160,6 +175,15 @@ class UKernelLibrary:
             [_vp, _i64, _i64] * 4 + [_i64, _i64, _vp, _vp, _i64, _i64, _i64,
                                      _i32, _i32, _i32, _u32, _vp])
         L.iree_uk_amd_mmt4d_dequant_unpack.restype = None
+        L.iree_uk_amd_mmt4d_epilogue_unpack.argtypes = (
+            [_vp, _i64, _i64] * 4 + [_i64, _i64, _vp, _vp, _vp, _i64, _i64, _i64,
+                                     _i32, _i32, _i32, _u32, _u32, _vp])
+        L.iree_uk_amd_mmt4d_epilogue_unpack.restype = None
+        L.iree_uk_amd_rmsnorm_pack.argtypes = (
+            [_vp, _i64, _i64] * 3 + [_vp, ctypes.c_float] + [_vp, _i64, _i64, _vp] + [_i64] * 6 + [_u32, _vp])
+        L.iree_uk_amd_rmsnorm_pack.restype = None
+        L.iree_uk_amd_gate_pack.argtypes = [_vp, _i64, _i64] * 3 + [_vp] + [_i64] * 6 + [_u32, _vp]
+        L.iree_uk_amd_gate_pack.restype = None
         L.iree_uk_conv_nchwc.argtypes = ([_vp, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _i64,
                                           _vp, _i64, _i64, _i64, _i64] + [_i64] * 7 +
                                          [_i32] * 4 + [_u32, _vp])
@@ -296,6 +320,43 @@ class UKernelLibrary:
             lhs, lhs_offset, lhs_stride0, rhs, rhs_offset, rhs_stride0, acc, acc_offset,
             acc_stride0, out, out_offset, out_stride0, out_size0, out_size1, row_scale,
             col_scale, M, N, K, M0, N0, K0, flags, cpu_data)
+        self._check()
+
+    def mmt4d_epilogue_unpack(self, lhs, lhs_offset, lhs_stride0, rhs, rhs_offset, rhs_stride0,
+                              residual, residual_offset, residual_stride0, out, out_offset,
+                              out_stride0, out_size0, out_size1, row_scale, col_scale, bias, M, N, K,
+                              M0, N0, K0, flags, epilogue_flags, cpu_data=None):
+        """mmt4d into a row-major f32, f16 or bf16 matrix: residual +
+        activation(product * row_scale * col_scale + bias). `epilogue_flags` is
+        OUT_TYPE_* | ACTIVATION_*; residual, scales and bias may be None."""
+        self.lib.iree_uk_amd_mmt4d_epilogue_unpack(
+            lhs, lhs_offset, lhs_stride0, rhs, rhs_offset, rhs_stride0, residual, residual_offset,
+            residual_stride0, out, out_offset, out_stride0, out_size0, out_size1, row_scale,
+            col_scale, bias, M, N, K, M0, N0, K0, flags, epilogue_flags, cpu_data)
+        self._check()
+
+    def rmsnorm_pack(self, inp, in_offset, in_stride0, residual, residual_offset, residual_stride0,
+                     sum, sum_offset, sum_stride0, weight, epsilon, out, out_offset, out_stride0,
+                     row_scale, in_size0, in_size1, out_size0, out_size1, out_size2, out_size3, flags,
+                     cpu_data=None):
+        """Root-mean-square norm of in + residual, row by row, into the tiles of
+        an mmt4d left-hand side, with a scale per row for the 8-bit types.
+        `flags` is IN_TYPE_* | OUT_TYPE_*; residual, sum and weight may be None."""
+        self.lib.iree_uk_amd_rmsnorm_pack(
+            inp, in_offset, in_stride0, residual, residual_offset, residual_stride0, sum, sum_offset,
+            sum_stride0, weight, epsilon, out, out_offset, out_stride0, row_scale, in_size0, in_size1,
+            out_size0, out_size1, out_size2, out_size3, flags, cpu_data)
+        self._check()
+
+    def gate_pack(self, gate, gate_offset, gate_stride0, up, up_offset, up_stride0, out, out_offset,
+                  out_stride0, row_scale, in_size0, in_size1, out_size0, out_size1, out_size2,
+                  out_size3, flags, cpu_data=None):
+        """activation(gate) * up into the tiles of an mmt4d left-hand side, with
+        a scale per row for the 8-bit types. `flags` is IN_TYPE_* | OUT_TYPE_* |
+        ACTIVATION_*; up may be None."""
+        self.lib.iree_uk_amd_gate_pack(
+            gate, gate_offset, gate_stride0, up, up_offset, up_stride0, out, out_offset, out_stride0,
+            row_scale, in_size0, in_size1, out_size0, out_size1, out_size2, out_size3, flags, cpu_data)
         self._check()
 
     def conv_nchwc(self, inp, input_offset, input_stride_n, input_stride_ic_outer,

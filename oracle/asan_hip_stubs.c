@@ -30,6 +30,26 @@ int uk_oracle_conv_nchwc(const void*, int64_t, int64_t, int64_t, int64_t, const 
 
 enum { kNotSupported = 801 }; /* hipErrorNotSupported */
 
+int iree_uk_amd_hip_launch_row_op(const iree_uk_amd_row_op_t* p, void* stream,
+                                  const char** kernel_name) {
+  (void)stream;
+  /* Touches what a kernel would: first and last bytes of every operand. */
+  *kernel_name = "row_op_touch";
+  const int es = (p->flags & IREE_UK_AMD_FLAG_IN_TYPE_MASK) == IREE_UK_AMD_FLAG_IN_TYPE_F32 ? 4 : 2;
+  const int os = p->row_scale ? 1 : es;
+  for (int64_t r = 0; r < p->rows && p->cols > 0; ++r) {
+    const char* x = (const char*)p->in + r * p->in_stride0 * es;
+    char last = x[p->cols * es - 1];
+    if (p->second) last ^= ((const char*)p->second + r * p->second_stride0 * es)[p->cols * es - 1];
+    if (p->sum) memset((char*)p->sum + r * p->sum_stride0 * es, last, (size_t)(p->cols * es));
+    if (p->weight) last ^= ((const char*)p->weight)[p->cols * es - 1];
+    if (p->row_scale) p->row_scale[r] = (float)last;
+  }
+  for (int64_t i = 0; i < p->M1; ++i)
+    memset((char*)p->out + i * p->out_stride0 * os, 7, (size_t)(p->K1 * p->M0 * p->K0 * os));
+  return 0;
+}
+
 int iree_uk_amd_hip_launch_pack(const iree_uk_pack_params_t* p, void* stream, int kernel_mode,
                                 const char** kernel_name) {
   (void)stream; (void)kernel_mode;

@@ -1,0 +1,229 @@
+"""iree_uk_amd_mmt4d_epilogue_unpack against its formula in 64 bits: the product
+(mmt4d.c:55-114 without an accumulator input), scales, bias, activation and
+residual. The reference has no such call.
+
+Operands are small integers, so that the products' sums are exact in 32 bits
+whatever their order; what is left are the roundings of 2^-24 of the
+conversion, of each factor, of the sums and of the activation, and one of the
+output's type."""
+import numpy as np
+import pytest
+import torch
+
+from iree_amd import ukernel as uk
+from test_gpu_row_ops import ACTS, HALF, U32, act64, act_slack
+
+# mmt4d type -> (operand kinds, bytes of what holds them)
+S8, F8, F16, BF16, F32 = (uk.MMT4D_TYPE_S8S8S32, uk.MMT4D_TYPE_F8E4M3FNF8E4M3FNF32, uk.MMT4D_TYPE_F16F16F32,
+                          uk.MMT4D_TYPE_BF16BF16F32, uk.MMT4D_TYPE_F32F32F32)
+TORCH = {S8: torch.int8, F8: torch.float8_e4m3fn, F16: torch.float16, BF16: torch.bfloat16, F32: torch.float32,
+         uk.MMT4D_TYPE_S16S16S32: torch.int16}
+OUTS = {"f32": (torch.float32, uk.OUT_TYPE_F32), "f16": (torch.float16, uk.OUT_TYPE_F16),
+        "bf16": (torch.bfloat16, uk.OUT_TYPE_BF16)}
+
+
+def tiled(x, t0, k0, t1, k1, dtype):
+    """A rows x k matrix of integers in tiles; what the tiles hold beyond it must not matter to it, so not zeros
+    beyond the rows; zeros beyond k."""
+    full = torch.full((t1 * t0, k1 * k0), 1.0)
+    full[:, x.shape[1]:] = 0
+    full[:x.shape[0], :x.shape[1]] = torch.from_numpy(x).float()
+    t = full.view(t1, t0, k1, k0).transpose(1, 2).contiguous()
+    return t.to(dtype).cuda()
+
+
+def run(lib, type_, rows, cols, k, M0, N0, K0, out, act, *, scales=True, bias=True, residual=None, pitch=0, offset=0,
+        flags=0, seed=0, capture=None):
+    """One call between guards, and its distance from the formula. `residual`: None, "own" or "in place"."""
+    rng = np.random.default_rng(seed)
+    M1, N1, K1 = -(-rows // M0), -(-cols // N0), -(-k // K0)
+    a = rng.integers(-4, 5, (rows, k)).astype(np.float64)
+    b = rng.integers(-4, 5, (cols, k)).astype(np.float64)
+    lhs, rhs = tiled(a, M0, K0, M1, K1, TORCH[type_]), tiled(b, N0, K0, N1, K1, TORCH[type_])
+    dt, fo = OUTS[out]
+    width = 10 / (6.0 * np.sqrt(max(k, 1)))
+    rs = torch.from_numpy((0.2 + rng.random(rows)) * 0.4).float().cuda() if scales else None
+    cs = torch.from_numpy((0.2 + rng.random(cols)) * width).float().cuda() if scales else None
+    bi = torch.from_numpy(rng.standard_normal(cols)).float().cuda() if bias else None
+    op, rp = cols + pitch, cols + 2 * pitch
+    buf = torch.from_numpy(rng.standard_normal(offset + rows * op + 9)).to(dt).cuda()
+    res = torch.from_numpy(2 * rng.standard_normal(offset + 2 + rows * rp)).to(dt).cuda()
+    before = buf.cpu().clone()
+    res_at, res_off = (buf, offset) if residual == "in place" else (res, offset + 1)
+    rp = op if residual == "in place" else rp
+
+    def at(t, pitch_, off):
+        return t[off:off + rows * pitch_].view(rows, pitch_)[:, :cols]
+
+    r64 = at(res_at, rp, res_off).cpu().double().numpy().copy() if residual else 0.0
+
+    def call():
+        lib.mmt4d_epilogue_unpack(
+            lhs.data_ptr(), 0, lhs[0].numel(), rhs.data_ptr(), 0, rhs[0].numel(),
+            res_at.data_ptr() if residual else None, res_off, rp, buf.data_ptr(), offset, op, rows, cols,
+            rs.data_ptr() if scales else None, cs.data_ptr() if scales else None, bi.data_ptr() if bias else None, M1, N1, K1,
+            M0, N0, K0, type_ | uk.MMT4D_ALLOW_GENERIC_FALLBACK_TILE_FUNCTION | flags, fo | ACTS[act])
+    if capture:
+        capture(call)
+    else:
+        call()
+        lib.synchronize()
+    name = (type_, rows, cols, k, M0, N0, K0, out, act, scales, bias, residual, pitch, lib.last_kernel_name())
+    z = a @ b.T
+    if scales:
+        z = z * rs.cpu().double().numpy()[:, None] * cs.cpu().double().numpy()
+    slack = np.abs(z) * 3 * U32
+    if bias:
+        z = z + bi.cpu().double().numpy()
+        slack = slack + np.abs(z) * U32
+    y = act64(z, act)
+    # (No activation is steeper than 1.13.)
+    slack = 1.13 * slack + act_slack(z, act)
+    want = r64 + y
+    half, tiny = HALF[out]
+    slack = slack + np.abs(want) * U32
+    got_buf = buf.cpu()
+    got = at(got_buf, op, offset).double().numpy()
+    off = np.abs(got - want) - (slack * (1 + half) + np.abs(want) * half + tiny)
+    assert off.max() <= 0, (name, off.max(), np.unravel_index(off.argmax(), off.shape))
+    at(got_buf, op, offset).copy_(at(before, op, offset))
+    assert torch.equal(got_buf, before), name   # nothing else was written
+    return name[-1]
+
+
+TILES = [(S8, 16, 16, 16), (S8, 32, 16, 8), (S8, 1, 16, 16), (S8, 16, 16, 2), (S8, 8, 6, 4), (F8, 16, 16, 32), (F8, 1, 16, 16),
+         (F16, 16, 16, 8), (F16, 1, 8, 16), (BF16, 16, 16, 8), (BF16, 16, 16, 2), (F32, 16, 16, 4), (F32, 16, 16, 1),
+         (uk.MMT4D_TYPE_S16S16S32, 16, 16, 2), (uk.MMT4D_TYPE_S16S16S32, 4, 6, 3)]
+MODES = [uk.KERNEL_MODE_AUTO, uk.KERNEL_MODE_GENERIC]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("mode", MODES)
+@pytest.mark.parametrize("type_,M0,N0,K0", TILES)
+def test_epilogue_of_small_and_ragged_sizes(gpu, type_, M0, N0, K0, mode):
+    """Every output type and activation, each part of the epilogue with and without, one row, one column,
+    K of less than a step and ragged, loose rows at odd addresses, the residual apart and in place."""
+    lib, _ = gpu
+    lib.set_kernel_mode(mode)
+    try:
+        i = 0
+        for rows, cols, k in [(1, 1, 5), (1, 70, 128), (3, 200, 1030), (17, 33, 64), (40, 150, 200), (70, 65, 512),
+                              (130, 129, 96), (16, 500, 768)]:
+            for out in OUTS:
+                act = list(ACTS)[i % 5]
+                run(lib, type_, rows, cols, k, M0, N0, K0, out, act, scales=i % 3 != 2, bias=i % 2 == 0,
+                    residual=(None, "own", "in place", "own")[i % 4], pitch=(0, 3, 4)[i % 3], offset=(0, 1)[i % 2], seed=i)
+                i += 1
+    finally:
+        lib.set_kernel_mode(uk.KERNEL_MODE_AUTO)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type_,M0,N0,K0", [(S8, 16, 16, 16), (F8, 16, 16, 32), (F16, 16, 16, 8), (BF16, 1, 16, 8),
+                                            (S8, 32, 16, 8)])
+@pytest.mark.parametrize("rows,cols,k", [
+    (1, 4096, 4096), (16, 1040, 16384), (64, 3000, 1024), (200, 4096, 2048), (300, 300, 8192), (1000, 1501, 777),
+    (2000, 40, 512), (40, 2000, 24576), (1030, 2050, 256), (2048, 4096, 128), (4100, 4200, 160), (4096, 8192, 64)])
+def test_epilogue_of_layer_sizes(gpu, type_, M0, N0, K0, rows, cols, k):
+    """The sizes at which the product's kernels change hands, from one row to several rounds of large blocks."""
+    lib, _ = gpu
+    i = rows + cols + k
+    for j, (out, residual) in enumerate([("bf16", "own"), ("f32", "in place"), ("f16", None)]):
+        run(lib, type_, rows, cols, k, M0, N0, K0, out, list(ACTS)[(i + j) % 5], bias=j != 1, scales=j != 2, residual=residual,
+            seed=j)
+
+
+@pytest.mark.gpu
+def test_epilogue_of_a_product_over_no_k(gpu):
+    """K == 0: what the epilogue makes of zeros."""
+    lib, _ = gpu
+    for out in OUTS:
+        for residual in (None, "own"):
+            run(lib, S8, 20, 33, 0, 16, 16, 16, out, "gelu", residual=residual)
+
+
+@pytest.mark.gpu
+def test_epilogue_passes_nan_scales_on(gpu):
+    """A row whose scale is NaN (one without an 8-bit form) is NaN throughout, its neighbours are not."""
+    lib, _ = gpu
+    for act in ACTS:
+        a = torch.ones(2, 4, 16, 16, dtype=torch.int8, device="cuda")
+        rs = torch.ones(32, device="cuda")
+        rs[5] = float("nan")
+        out = torch.zeros(32, 48, device="cuda")
+        b = torch.ones(3, 4, 16, 16, dtype=torch.int8, device="cuda")
+        lib.mmt4d_epilogue_unpack(a.data_ptr(), 0, a.stride(0), b.data_ptr(), 0, b.stride(0), None, 0, 0, out.data_ptr(), 0, 48,
+                                  32, 48, rs.data_ptr(), None, None, 2, 3, 4, 16, 16, 16, S8, uk.OUT_TYPE_F32 | ACTS[act])
+        lib.synchronize()
+        assert bool(out[5].isnan().all()) and not out[:5].isnan().any() and not out[6:].isnan().any(), act
+
+
+@pytest.mark.gpu
+def test_epilogue_in_a_captured_graph(gpu):
+    """Captured and replayed on a side stream, with eager calls between, for the kernels that own a workspace
+    outside a graph, too."""
+    lib, _ = gpu
+    s = torch.cuda.Stream()
+
+    def capture(call):
+        torch.cuda.synchronize()
+        lib.set_stream(s.cuda_stream)
+        lib.set_pointer_mode(uk.POINTER_MODE_DEVICE)
+        try:
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=s):
+                call()
+            for _ in range(3):
+                g.replay()
+                torch.cuda.synchronize()
+            call()
+            g.replay()
+            torch.cuda.synchronize()
+        finally:
+            lib.set_stream(None)
+            lib.set_pointer_mode(uk.POINTER_MODE_AUTO)
+
+    for type_, M0, N0, K0, rows, cols, k in [(S8, 16, 16, 16, 16, 512, 16384), (BF16, 16, 16, 2, 200, 300, 512),
+                                             (F8, 16, 16, 32, 300, 300, 8192), (F32, 16, 16, 1, 40, 50, 60)]:
+        for out in ("bf16", "f32"):
+            run(lib, type_, rows, cols, k, M0, N0, K0, out, "silu", residual="own", capture=capture)
+
+
+@pytest.mark.gpu
+def test_epilogue_on_host_memory(gpu):
+    lib, _ = gpu
+    rng = np.random.default_rng(4)
+    a = rng.integers(-9, 9, (20, 64)).astype(np.int8)
+    b = rng.integers(-9, 9, (33, 64)).astype(np.int8)
+    bias = rng.standard_normal(33).astype(np.float32)
+    res = rng.standard_normal((20, 40)).astype(np.float32)
+    rs = rng.random(20).astype(np.float32)
+    want = np.maximum((a.astype(np.float64) @ b.T.astype(np.float64)) * rs[:, None] + bias, 0) + res[:, :33]
+    for out in (np.full((20, 36), 7, np.float32), res):   # apart, and in place
+        pitch = out.shape[1]
+        lib.mmt4d_epilogue_unpack(a.ctypes.data, 0, 64, b.ctypes.data, 0, 64, res.ctypes.data, 0, 40, out.ctypes.data, 0, pitch,
+                                  20, 33, rs.ctypes.data, None, bias.ctypes.data, 20, 33, 4, 1, 1, 16,
+                                  S8 | uk.MMT4D_ALLOW_GENERIC_FALLBACK_TILE_FUNCTION, uk.OUT_TYPE_F32 | uk.ACTIVATION_RELU)
+        assert np.abs(out[:, :33] - want).max() <= 8 * U32 * np.abs(want).max()
+        if out is not res:
+            assert (out[:, 33:] == 7).all()
+
+
+def test_epilogue_refusals(lib):
+    """Needs no device."""
+    lib.raise_on_violation(True)
+
+    def call(flags=S8, ep=uk.OUT_TYPE_BF16, rows=16, cols=16, M=1, stride=16, rstride=0):
+        lib.mmt4d_epilogue_unpack(None, 0, 0, None, 0, 0, None, 0, rstride, None, 0, stride, rows, cols, None, None, None, M, 1,
+                                  1, 16, 16, 16, flags, ep)
+
+    for kw in [dict(flags=uk.MMT4D_TYPE_F16F16F16 | uk.MMT4D_SKIP_INTERMEDIATE_ROUNDINGS), dict(flags=0),
+               dict(flags=S8 | uk.MMT4D_ACCUMULATE), dict(ep=0), dict(ep=uk.OUT_TYPE_S8), dict(ep=uk.OUT_TYPE_F8E4M3FN),
+               dict(ep=uk.OUT_TYPE_F32 | 0x500), dict(ep=uk.OUT_TYPE_F32 | uk.IN_TYPE_F32), dict(ep=0x1010), dict(rows=17),
+               dict(cols=17), dict(rows=-1), dict(stride=-16), dict(rstride=-1),
+               dict(flags=uk.MMT4D_TYPE_S16S8S32)]:
+        with pytest.raises(uk.ContractViolation):
+            call(**kw)
+    call(rows=0)
+    call(cols=0)
+    call(rows=0, M=0)
