@@ -23,6 +23,11 @@ int launch_f32_rb4(const Problem& p, int forced, hipStream_t stream, const char*
 int launch_f32_rb8(const Problem& p, int forced, hipStream_t stream, const char** name);
 int launch_f32_rb16(const Problem& p, int forced, hipStream_t stream, const char** name);
 int launch_f8_rb16(const Problem& p, int forced, hipStream_t stream, const char** name);
+int launch_s8ep_rb8(const Problem& p, int forced, hipStream_t stream, const char** name);
+int launch_s8ep_rb16(const Problem& p, int forced, hipStream_t stream, const char** name);
+int launch_f16ep_rb16(const Problem& p, int forced, hipStream_t stream, const char** name);
+int launch_bf16ep_rb16(const Problem& p, int forced, hipStream_t stream, const char** name);
+int launch_f8ep_rb16(const Problem& p, int forced, hipStream_t stream, const char** name);
 #undef UK_DECLARE_ROW_CLASSES
 #define UK_DEFINE_BY_ROW_BYTES(T)                                                            \
   inline int launch_##T(const Problem& p, int forced, hipStream_t stream, const char** name) { \
@@ -51,6 +56,21 @@ inline int launch_f8(const Problem& p, int forced, hipStream_t stream, const cha
   return p.rb >= 16 ? launch_f8_rb16(p, forced, stream, name) : -1;
 }
 int launch_s8s4(const Problem& p, hipStream_t stream, const char** name);
+int launch_s8s4ep(const Problem& p, hipStream_t stream, const char** name);
+// Products that end in an epilogue: the types of quantized and 16-bit layers, in tile rows
+// of 16 bytes and more, 8-bit integers of 8 bytes, too. (The others are a product into f32
+// and the epilogue apart: launch_epilogue_apart.)
+inline int launch_with_epilogue(Elem e, const Problem& p, hipStream_t stream, const char** name) {
+  switch (e) {
+    case Elem::kS8S4: return launch_s8s4ep(p, stream, name);
+    case Elem::kS8:
+      return p.rb == 8 ? launch_s8ep_rb8(p, 0, stream, name) : p.rb >= 16 ? launch_s8ep_rb16(p, 0, stream, name) : -1;
+    case Elem::kF16: return p.rb >= 16 ? launch_f16ep_rb16(p, 0, stream, name) : -1;
+    case Elem::kBF16: return p.rb >= 16 ? launch_bf16ep_rb16(p, 0, stream, name) : -1;
+    case Elem::kF8: return p.rb >= 16 ? launch_f8ep_rb16(p, 0, stream, name) : -1;
+    default: return -1;
+  }
+}
 int launch_s16(const Problem& p, int forced, hipStream_t stream, const char** name);
 }  // namespace uk_mfma
 
@@ -122,6 +142,7 @@ struct OwnedWorkspaces : std::vector<OwnedWorkspace> {
 constexpr size_t kMaxOwnedWorkspaces = 8;
 thread_local OwnedWorkspaces g_workspaces;
 thread_local OwnedWorkspaces g_expand_workspaces;   // s4 weights expanded to s8 (n_counters unused)
+thread_local OwnedWorkspaces g_product_workspaces;  // products in f32 in front of an epilogue (n_counters unused)
 thread_local bool g_no_alloc = false;
 thread_local int g_k_slices = 0;
 thread_local int g_last_k_slices = 1;
@@ -334,14 +355,14 @@ void retile_rows(const char* src, int64_t src_stride, int panels, int R0, int rb
 #undef UK_RETILE
 }
 
-int acquire_expand_workspace(size_t bytes, hipStream_t stream, char** base_out) {
+namespace {
+int acquire_from(OwnedWorkspaces& pool, size_t bytes, hipStream_t stream, char** base_out) {
   if (g_no_alloc || bytes == 0 || bytes > ((size_t)2 << 30)) return 1;
   hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
   if (hipStreamIsCapturing(stream, &capture) != hipSuccess) { (void)hipGetLastError(); return 1; }
   if (capture != hipStreamCaptureStatusNone) return 1;
   int dev = 0;
   if (hipGetDevice(&dev) != hipSuccess) return 1;
-  OwnedWorkspaces& pool = g_expand_workspaces;
   const uint64_t now = ++pool.uses;
   for (OwnedWorkspace& w : pool) {
     if (w.device == dev && w.stream == stream && w.partial_bytes >= bytes) {
@@ -377,6 +398,14 @@ int acquire_expand_workspace(size_t bytes, hipStream_t stream, char** base_out) 
   *base_out = base;
   return 0;
 }
+}  // namespace
+
+int acquire_expand_workspace(size_t bytes, hipStream_t stream, char** base_out) {
+  return acquire_from(g_expand_workspaces, bytes, stream, base_out);
+}
+int acquire_product_workspace(size_t bytes, hipStream_t stream, char** base_out) {
+  return acquire_from(g_product_workspaces, bytes, stream, base_out);
+}
 
 }  // namespace uk_mfma
 
@@ -384,13 +413,14 @@ extern "C" IREE_UK_AMD_EXPORT int64_t iree_uk_amd_workspace_bytes(void) {
   int64_t total = 0;
   for (const OwnedWorkspace& w : g_workspaces) total += (int64_t)w.partial_bytes + (int64_t)w.n_counters * 4;
   for (const OwnedWorkspace& w : g_expand_workspaces) total += (int64_t)w.partial_bytes;
+  for (const OwnedWorkspace& w : g_product_workspaces) total += (int64_t)w.partial_bytes;
   return total;
 }
 
 extern "C" IREE_UK_AMD_EXPORT int iree_uk_amd_release_workspaces(void) {
   int status = 0, current = 0;
   (void)hipGetDevice(&current);
-  for (OwnedWorkspaces* pool : {&g_workspaces, &g_expand_workspaces}) {
+  for (OwnedWorkspaces* pool : {&g_workspaces, &g_expand_workspaces, &g_product_workspaces}) {
     for (OwnedWorkspace& w : *pool) {
       if (!w.base) continue;
       (void)hipSetDevice(w.device);
@@ -508,6 +538,11 @@ extern "C" int iree_uk_amd_hip_launch_mmt4d_mfma(const iree_uk_mmt4d_params_t* p
     if (!iree_uk_amd_hip_mmt4d_mfma_supported(p->M0, p->N0, p->K0, p->flags)) return -1;
   }
   if (p->K == 0) return -1;  // zero fill only: the generic kernel does it
+  const bool epilogue = rowmajor && rowmajor->epilogue;
+  if (epilogue) {
+    ob = (rowmajor->epilogue_flags & IREE_UK_AMD_FLAG_OUT_TYPE_MASK) == IREE_UK_AMD_FLAG_OUT_TYPE_F32 ? 4 : 2;
+    if ((uintptr_t)rowmajor->residual & (uintptr_t)(ob - 1)) return -1;
+  }
   uk_mfma::note_k_slices(1);
   hipStream_t stream = (hipStream_t)stream_v;
   uk_mfma::Problem pr;
@@ -539,7 +574,7 @@ extern "C" int iree_uk_amd_hip_launch_mmt4d_mfma(const iree_uk_mmt4d_params_t* p
   pr.dequant = false;
   pr.row_scale = pr.col_scale = nullptr;
   if (rowmajor && rowmajor->dequant) {
-    if (ob != 4) return -1;
+    if (ob != 4 && !epilogue) return -1;
     pr.dequant = true;
     pr.row_scale = rowmajor->row_scale;
     pr.col_scale = rowmajor->col_scale;
@@ -571,6 +606,17 @@ extern "C" int iree_uk_amd_hip_launch_mmt4d_mfma(const iree_uk_mmt4d_params_t* p
   while ((1 << pr.lrb) < pr.rb) ++pr.lrb;
   pr.accumulate = (p->flags & IREE_UK_FLAG_MMT4D_ACCUMULATE) != 0;
   pr.cus = uk_mfma::compute_units();
+  pr.ep = uk_mfma::Epilogue{};
+  if (epilogue) {
+    pr.ep.out_type = rowmajor->epilogue_flags & IREE_UK_AMD_FLAG_OUT_TYPE_MASK;
+    pr.ep.act = rowmajor->epilogue_flags & IREE_UK_AMD_FLAG_ACTIVATION_MASK;
+    pr.ep.out_bytes = (uint32_t)ob;
+    pr.ep.out_pitch = pr.out_sm0;
+    pr.ep.bias = rowmajor->bias;
+    pr.ep.residual = (const char*)rowmajor->residual;
+    pr.ep.residual_pitch = rowmajor->residual_stride0 * ob;
+    return uk_mfma::launch_with_epilogue(e, pr, stream, kernel_name);
+  }
   switch (e) {
     case Elem::kS8S4: return uk_mfma::launch_s8s4(pr, stream, kernel_name);
     case Elem::kS16: return uk_mfma::launch_s16(pr, forced_variant, stream, kernel_name);
@@ -581,6 +627,7 @@ extern "C" int iree_uk_amd_hip_launch_mmt4d_mfma(const iree_uk_mmt4d_params_t* p
     case Elem::kF32: return uk_mfma::launch_f32(pr, forced_variant, stream, kernel_name);
     case Elem::kF16F16: return uk_mfma::launch_f16f16(pr, forced_variant, stream, kernel_name);
     case Elem::kBF16BF16: return uk_mfma::launch_bf16bf16(pr, forced_variant, stream, kernel_name);
+    default: return -1;
   }
   return -1;
 }

@@ -1,0 +1,83 @@
+// What lies between the sums of a matrix-core product and the row-major matrix of
+// iree_uk_amd_mmt4d_epilogue_unpack: scales, bias, activation, residual, and the one
+// rounding to the matrix's type. Device code of the instances for Elem::k...Ep.
+#ifndef IREE_UK_AMD_MMT4D_MFMA_EPILOGUE_H_
+#define IREE_UK_AMD_MMT4D_MFMA_EPILOGUE_H_
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "uk_activation.h"
+
+namespace uk_mfma {
+
+struct Epilogue {
+  uint32_t out_type, act;     // IREE_UK_AMD_FLAG_OUT_TYPE_*, IREE_UK_AMD_FLAG_ACTIVATION_*
+  uint32_t out_bytes;         // of an element
+  uint32_t swapped;           // mmt4d_mfma_thin.h: the kernel's rows are the caller's columns
+  int64_t out_pitch;          // bytes between rows of the matrix
+  const float* bias;          // of the caller's columns; null: none
+  const char* residual;       // null: none
+  int64_t residual_pitch;     // bytes
+};
+
+// N consecutive elements of a row of the out type, at any address of its elements.
+template <typename F, int N>
+struct RowPiece {
+  typedef typename F::T V __attribute__((ext_vector_type(N)));
+  typedef V Any __attribute__((aligned(sizeof(typename F::T))));
+};
+
+// f(F32{}), f(F16{}) or f(BF16{}), by the out type (the same in all lanes).
+template <typename Body>
+__device__ __forceinline__ void by_out_type(const Epilogue& ep, Body&& f) {
+  if (ep.out_type == IREE_UK_AMD_FLAG_OUT_TYPE_BF16) f(uk::BF16{});
+  else if (ep.out_type == IREE_UK_AMD_FLAG_OUT_TYPE_F16) f(uk::F16{});
+  else f(uk::F32{});
+}
+
+// Elements (row, col) .. (row, col + N - 1) of the matrix, of which `left` exist (N and
+// more: all): the residual's elements as f32, zeros where there is none.
+template <int N>
+__device__ __forceinline__ void load_residual(const Epilogue& ep, int row, int col, int left, float (&v)[N]) {
+#pragma unroll
+  for (int e = 0; e < N; ++e) v[e] = 0.0f;
+  if (!ep.residual || left <= 0) return;
+  const char* p = ep.residual + (int64_t)row * ep.residual_pitch + (int64_t)col * ep.out_bytes;
+  by_out_type(ep, [&](auto type) __attribute__((always_inline)) {
+    using F = decltype(type);
+    if (left >= N) {
+      const auto x = *reinterpret_cast<const typename RowPiece<F, N>::Any*>(p);
+#pragma unroll
+      for (int e = 0; e < N; ++e) v[e] = F::to_f32(x[e]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        if (e < left) v[e] = F::to_f32(reinterpret_cast<const typename F::T*>(p)[e]);
+    }
+  });
+}
+
+// The same elements, rounded and stored.
+template <int N>
+__device__ __forceinline__ void store_row(const Epilogue& ep, char* out, int row, int col, int left, const float (&v)[N]) {
+  if (left <= 0) return;
+  char* p = out + (int64_t)row * ep.out_pitch + (int64_t)col * ep.out_bytes;
+  by_out_type(ep, [&](auto type) __attribute__((always_inline)) {
+    using F = decltype(type);
+    if (left >= N) {
+      typename RowPiece<F, N>::V x;
+#pragma unroll
+      for (int e = 0; e < N; ++e) x[e] = F::from_f32(v[e]);
+      *reinterpret_cast<typename RowPiece<F, N>::Any*>(p) = x;
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        if (e < left) reinterpret_cast<typename F::T*>(p)[e] = F::from_f32(v[e]);
+    }
+  });
+}
+
+}  // namespace uk_mfma
+
+#endif  // IREE_UK_AMD_MMT4D_MFMA_EPILOGUE_H_

@@ -62,6 +62,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "mmt4d_mfma_epilogue.h"
 #include "uk_device_common.h"
 #include "uk_float_convert.h"
 
@@ -87,7 +88,14 @@ typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 // kS16: s16 x s16 -> s32 as four 8-bit integer products per element pair (the
 // hardware has no 16-bit integer matrix instruction); served by the LDS-direct
 // pipeline only (PIPE 5 below, which describes the arithmetic).
-enum class Elem { kS8, kF16, kBF16, kF8, kF32, kF16F16, kBF16BF16, kS8S4, kS16 };
+// k...Ep: the same operands and sums, whose results go through an epilogue
+// (mmt4d_mfma_epilogue.h) into a row-major matrix.
+enum class Elem { kS8, kF16, kBF16, kF8, kF32, kF16F16, kBF16BF16, kS8S4, kS16, kS8Ep, kF16Ep, kBF16Ep, kF8Ep, kS8S4Ep };
+
+template <Elem E>
+constexpr bool has_epilogue() {
+  return E == Elem::kS8Ep || E == Elem::kF16Ep || E == Elem::kBF16Ep || E == Elem::kF8Ep || E == Elem::kS8S4Ep;
+}
 
 typedef uint16_t v4u16 __attribute__((ext_vector_type(4)));
 typedef uint32_t v2u32 __attribute__((ext_vector_type(2)));
@@ -221,6 +229,12 @@ template <> struct ElemTraits<Elem::kF16F16> : ElemTraits<Elem::kF16> {
 template <> struct ElemTraits<Elem::kBF16BF16> : ElemTraits<Elem::kBF16> {
   using Out = Out16<8>;
 };
+// (Out is not used for the matrix of an epilogue; kernels are chosen as for 4-byte results.)
+template <> struct ElemTraits<Elem::kS8Ep> : ElemTraits<Elem::kS8> {};
+template <> struct ElemTraits<Elem::kF16Ep> : ElemTraits<Elem::kF16> {};
+template <> struct ElemTraits<Elem::kBF16Ep> : ElemTraits<Elem::kBF16> {};
+template <> struct ElemTraits<Elem::kF8Ep> : ElemTraits<Elem::kF8> {};
+template <> struct ElemTraits<Elem::kS8S4Ep> : ElemTraits<Elem::kS8S4> {};
 
 // LDS-direct loads (PIPE 5): address-space-qualified pointers for the builtin,
 // and the wait for "at most N vector memory operations still in flight" (the
@@ -348,6 +362,9 @@ struct Args {
   uint32_t slice_steps, longer_slices;
   // mmt4d_mfma_thin.h only: `band` counts block columns, not rows.
   uint32_t column_bands;
+  // Elem::k...Ep only: what becomes of the scaled sums (`out` is then the first
+  // element of a row-major matrix, from this problem's origin).
+  Epilogue ep;
 };
 
 // The last fields of Args from those before.
@@ -429,6 +446,26 @@ __device__ __forceinline__ void block_of_workgroup(uint32_t wg, const Args& a,
   *bm = (int)(b * a.band + (in_band - col * rows));
   *bn = (int)col;
 }
+
+template <Elem E, int TM, int TN, int WGM, int WGN, int NKK, int PIPE, bool SLICED = false>
+struct Shape {
+  static constexpr int NCH = NKK * ElemTraits<E>::kHalves * 4;
+  static constexpr int KS = NCH * 16;
+  static constexpr int BM = WGM * TM * 16;
+  static constexpr int BN = WGN * TN * 16;
+  static constexpr size_t kOperandLdsBytes =
+      (PIPE == 5 && ElemTraits<E>::kHalves == 2)
+          ? ring_slots<E, BM, BN, SLICED>() * (size_t)(BM + BN) * 64   // a ring of half-step slots
+          : (PIPE == 5 ? stages5<SLICED>() : PIPE == 0 || PIPE == 4 ? 2 : 3) *
+                (size_t)(PIPE == 2 || PIPE == 3 ? BM : BM + BN) * KS;
+  // Row blocks of a wave that its epilogue has in LDS at a time: all, or as many as leave
+  // the workgroup with what its operands take (half: 256x256 blocks, which share a unit
+  // with no other anyway, 64 KB a pass of 16).
+  static constexpr size_t kEpilogueBlockBytes = (size_t)WGM * WGN * TN * 1024;
+  static constexpr int kEpilogueBlocks = TM * kEpilogueBlockBytes <= 64 * 1024 ? TM : TM / 2;
+  static constexpr size_t kEpilogueLdsBytes = has_epilogue<E>() ? kEpilogueBlocks * kEpilogueBlockBytes : 0;
+  static constexpr size_t kLdsBytes = kOperandLdsBytes > kEpilogueLdsBytes ? kOperandLdsBytes : kEpilogueLdsBytes;
+};
 
 // TM x TN accumulator blocks per wave, WGM x WGN waves per workgroup, NKK MFMA
 // K-groups per pipeline step, PIPE as described at the top of this file.
@@ -703,7 +740,7 @@ void mmt4d_mfma_kernel(Args a) {
   // were too long for the compiler to unroll, and their accumulators, indexed by
   // a running number, lived in scratch memory all through the K loop (bf16 4616 x
   // 4207 x 560 514 us, now 57; 4096^3 2495 us, now 103).
-  if (a.accumulate) {
+  if (!has_epilogue<E>() && a.accumulate) {
     if constexpr (OB == 2) {
       v2u32 bits[TM][TN];
 #pragma unroll
@@ -1644,7 +1681,10 @@ void mmt4d_mfma_kernel(Args a) {
         else step_body(s, std::integral_constant<int, 2 * decltype(phase_c)::value % RING>{},
                        std::bool_constant<decltype(phase_c)::value % 2 != 0>{});
       };
-      if constexpr (TAIL && !S16) {
+      // (256x256 blocks that end in an epilogue, too: unrolled they came out with 122
+      // registers in scratch memory, as the blocks of the other types and without an
+      // epilogue do not; f8 2048 x 8192 x 28672 1627 us, so 0.)
+      if constexpr ((TAIL || (has_epilogue<E>() && TM * TN >= 32)) && !S16) {
         // Rolled: the test of every load against the end of K, in every copy of
         // the unrolled loop, asked for more registers than there are (f8 4096 x
         // 4096 x 4001: 256 us against 55, which is also what K = 4096 takes unrolled).
@@ -1770,6 +1810,71 @@ void mmt4d_mfma_kernel(Args a) {
       for (int tn = 0; tn < TN; ++tn) acc[tm][tn] += acc_odd[tm][tn];
   }
   // ---- epilogue -----------------------------------------------------------
+  if constexpr (has_epilogue<E>()) {
+    // Through LDS, which the operands no longer need: a wave puts the sums of some of its
+    // rows there as they lie in its lanes and takes them out again eight columns of one
+    // row a lane, in a loop that is rolled. A lane's columns are then the same in every
+    // round (their scales and biases are loaded once), a 16-bit row of the wave's block is
+    // stored in whole 32 to 128 bytes, and the activations' code exists once, not once for
+    // each of the 128 sums of a lane. The 16-byte chunks of a row change places with its
+    // number, so that neither the writes nor the reads meet on a bank.
+    using SH = Shape<E, TM, TN, WGM, WGN, NKK, PIPE, SLICED>;
+    constexpr int COLS = TN * 16, CH = COLS / 4, PASS = SH::kEpilogueBlocks, ROWS = PASS * 16;
+    constexpr int LPR = COLS / 8, RPI = 64 / LPR;   // lanes a row, rows a round
+    static_assert(TM % PASS == 0 && ROWS % RPI == 0, "whole passes and rounds");
+    __syncthreads();   // (every operand has been read, every LDS-direct load has landed)
+    // (The lane's number anew, so that none of this is kept in registers through the K loop.)
+    uint32_t own_lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(own_lane));
+    const uint32_t q = own_lane >> 4, r = own_lane & 15;
+    const int lane = (int)own_lane;
+    v4f* mine = reinterpret_cast<v4f*>(lds) + wave * (ROWS * CH);
+    const int row_origin = pm0 * a.M0, col_origin = pn0 * a.N0;
+    const int rows_here = min(a.bpm * a.M0, a.out_rows - row_origin);
+    const int c8 = lane % LPR, row0 = lane / LPR;
+    const int col = wn * COLS + c8 * 8;
+    const int left = min(a.bpn * a.N0, a.out_cols - col_origin) - col;
+    float sn[8], bias[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int c = max(min(col_origin + col + e, a.out_cols - 1), 0);   // (beyond: never stored)
+      sn[e] = a.col_scale ? a.col_scale[c] : 1.0f;
+      bias[e] = a.ep.bias ? a.ep.bias[c] : 0.0f;
+    }
+#pragma unroll
+    for (int pass = 0; pass < TM / PASS; ++pass) {
+#pragma unroll
+      for (int t = 0; t < PASS; ++t)
+#pragma unroll
+        for (int tn = 0; tn < TN; ++tn) {
+          const uint32_t row = (uint32_t)t * 16 + r;
+          mine[row * CH + ((uint32_t)(tn * 4 + q) ^ (row & (CH - 1)))] =
+              __builtin_convertvector(acc[pass * PASS + t][tn], v4f);
+        }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma nounroll
+      for (int i = 0; i < ROWS; i += RPI) {
+        const int row = i + row0;
+        const int block_row = (wm * TM + pass * PASS) * 16 + row;
+        if (block_row < rows_here && left > 0) {
+          const int mrow = row_origin + block_row, mcol = col_origin + col;
+          float rv[8], z[8];
+          load_residual(a.ep, mrow, mcol, left, rv);
+          const float sm = a.row_scale ? a.row_scale[mrow] : 1.0f;
+          const uint32_t turn = (uint32_t)row & (CH - 1);
+          const v4f lo = mine[row * CH + ((2 * c8) ^ turn)], hi = mine[row * CH + ((2 * c8 + 1) ^ turn)];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) z[e] = (e < 4 ? lo[e] : hi[e - 4]) * sm * sn[e] + bias[e];
+          uk::activate_all(z, a.ep.act);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) z[e] += rv[e];
+          store_row(a.ep, a.out, mrow, mcol, left, z);
+        }
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+    return;
+  }
   if constexpr (OB == 4) {
     if (a.dequant) {
       // Scales of this lane's rows and columns; indices beyond the matrix are
@@ -1839,19 +1944,6 @@ void mmt4d_mfma_kernel(Args a) {
                     [&](int tm, int tn, int e, char* p) { Out::store1(p, acc[tm][tn][e]); });
   }
 }
-
-template <Elem E, int TM, int TN, int WGM, int WGN, int NKK, int PIPE, bool SLICED = false>
-struct Shape {
-  static constexpr int NCH = NKK * ElemTraits<E>::kHalves * 4;
-  static constexpr int KS = NCH * 16;
-  static constexpr int BM = WGM * TM * 16;
-  static constexpr int BN = WGN * TN * 16;
-  static constexpr size_t kLdsBytes =
-      (PIPE == 5 && ElemTraits<E>::kHalves == 2)
-          ? ring_slots<E, BM, BN, SLICED>() * (size_t)(BM + BN) * 64   // a ring of half-step slots
-          : (PIPE == 5 ? stages5<SLICED>() : PIPE == 0 || PIPE == 4 ? 2 : 3) *
-                (size_t)(PIPE == 2 || PIPE == 3 ? BM : BM + BN) * KS;
-};
 
 }  // namespace uk_mfma
 

@@ -43,6 +43,7 @@ struct Problem {
   int32_t M1, N1, K1, M0, N0;
   int32_t rb, lrb;  // bytes per tile row and its log2
   bool accumulate;
+  Epilogue ep;      // Elem::k...Ep
   int32_t cus;      // compute units of the device, 0: the query failed, as the launch will (asked for once a call)
 };
 
@@ -115,6 +116,7 @@ int launch_variant(const Problem& p, int kt_begin, int kt_count, bool accumulate
   a.dequant = p.dequant && kt_begin + kt_count == p.K1;
   a.row_scale = p.row_scale;
   a.col_scale = p.col_scale;
+  a.ep = p.ep;
   // Block rows per rasterization band: an XCD's 32 resident workgroups should
   // cover a near-square patch of the output (4 x 8 blocks of 256x256, 8 x 4 of
   // 128x512: 3072 operand rows either way).
@@ -360,7 +362,7 @@ int launch_thin(const Problem& caller, bool swapped, hipStream_t stream, bool al
   }
   constexpr int KS = 64 * ElemTraits<E>::kHalves;
   constexpr int OB = OBYTES;
-  constexpr bool S4 = E == Elem::kS8S4;  // rb, lrb describe the LHS; RHS rows are half as wide
+  constexpr bool S4 = E == Elem::kS8S4 || E == Elem::kS8S4Ep;  // rb, lrb describe the LHS; RHS rows are half as wide
   if (p.rb > KS || p.rb < (S4 ? 16 : std::min(RBC, 8))) return -1;
   const int64_t k_bytes = (int64_t)p.K1 << p.lrb;
   const bool tail = k_bytes % KS != 0;
@@ -395,6 +397,8 @@ int launch_thin(const Problem& caller, bool swapped, hipStream_t stream, bool al
   a.acc_sn0 = (uint32_t)(swapped ? p.acc_sm0 : OBYTES);
   a.acc_spn = (uint32_t)p.acc_spn;
   a.dequant = p.dequant; a.row_scale = p.row_scale; a.col_scale = p.col_scale;
+  a.ep = p.ep;
+  a.ep.swapped = swapped;
   a.col_scale_first = swapped;
   auto vector_ok = [&](const char* base, int64_t stride, int64_t sm0, int64_t spn) {
     const bool contiguous4 = p.N0 % 4 == 0 || spn == (int64_t)p.N0 * OB;
@@ -566,7 +570,11 @@ inline int finish_k(int st) { return st < 0 ? (int)hipErrorUnknown : st; }
 template <Elem E, int RBC>
 int launch_slices(const Problem& p, int slices, hipStream_t stream) {
   // 16-bit results: the sums of the slices are 32-bit floats like those of a block.
-  constexpr Elem P = E == Elem::kF16F16 ? Elem::kF16 : E == Elem::kBF16BF16 ? Elem::kBF16 : E;
+  constexpr Elem P = E == Elem::kF16F16 || E == Elem::kF16Ep       ? Elem::kF16
+                     : E == Elem::kBF16BF16 || E == Elem::kBF16Ep ? Elem::kBF16
+                     : E == Elem::kS8Ep                           ? Elem::kS8
+                     : E == Elem::kF8Ep                           ? Elem::kF8
+                                                                  : E;
   using Out = typename ElemTraits<E>::Out;
   constexpr int KS = 64 * ElemTraits<E>::kHalves;
   const int64_t k_bytes = (int64_t)p.K1 << p.lrb;
@@ -608,6 +616,7 @@ int launch_slices(const Problem& p, int slices, hipStream_t stream) {
   s.acc = p.accumulate ? p.acc : nullptr; s.acc_stride = p.acc_stride;
   s.acc_sm0 = (uint32_t)p.acc_sm0; s.acc_spn = (uint32_t)p.acc_spn;
   s.dequant = p.dequant; s.row_scale = p.row_scale; s.col_scale = p.col_scale;
+  s.ep = p.ep;
   constexpr int OB = Out::kOutBytes;
   auto vector_ok = [&](const char* base, int64_t stride, int64_t sm0, int64_t spn) {
     const bool contiguous4 = p.N0 % 4 == 0 || spn == (int64_t)p.N0 * OB;
@@ -618,7 +627,8 @@ int launch_slices(const Problem& p, int slices, hipStream_t stream) {
   s.vec = vector_ok(p.out, p.out_stride, p.out_sm0, p.out_spn) &&
           (!p.accumulate || vector_ok(p.acc, p.acc_stride, p.acc_sm0, p.acc_spn));
   const dim3 grid((uint32_t)uk::ceil_div(s.cols, 4 * kSumThreads), (uint32_t)s.rows);
-  uk::launch(2, mmt4d_sum_slices_kernel<typename ElemTraits<E>::Acc, Out>, grid, dim3(kSumThreads), 0, stream, s);
+  uk::launch(2, mmt4d_sum_slices_kernel<typename ElemTraits<E>::Acc, Out, has_epilogue<E>()>, grid, dim3(kSumThreads), 0,
+             stream, s);
   return finish_k((int)hipGetLastError());
 }
 
@@ -1115,6 +1125,8 @@ int launch_class(const Problem& p, int forced, hipStream_t stream, const char** 
         q.out = p.out + (int64_t)main_n * p.out_spn;
         q.acc = p.acc + (int64_t)main_n * p.acc_spn;
         if (p.col_scale) q.col_scale = p.col_scale + (int64_t)main_n * p.N0;
+        if (p.ep.bias) q.ep.bias = p.ep.bias + (int64_t)main_n * p.N0;
+        if (p.ep.residual) q.ep.residual = p.ep.residual + (int64_t)main_n * p.N0 * p.ep.out_bytes;
         q.out_cols = p.out_cols - (int64_t)main_n * p.N0;
         q.N1 = p.N1 - main_n;
         st = launch_class<E, RBC>(q, 0, stream, &strip_name);
@@ -1128,6 +1140,7 @@ int launch_class(const Problem& p, int forced, hipStream_t stream, const char** 
         q.out = p.out + (int64_t)main_m * p.out_stride;
         q.acc = p.acc + (int64_t)main_m * p.acc_stride;
         if (p.row_scale) q.row_scale = p.row_scale + (int64_t)main_m * p.M0;
+        if (p.ep.residual) q.ep.residual = p.ep.residual + (int64_t)main_m * p.M0 * p.ep.residual_pitch;
         q.out_rows = p.out_rows - (int64_t)main_m * p.M0;
         q.out_cols = own_cols;
         q.M1 = p.M1 - main_m;
@@ -1150,10 +1163,13 @@ int launch_class(const Problem& p, int forced, hipStream_t stream, const char** 
   // SKIP_INTERMEDIATE_ROUNDINGS semantics): a second launch would continue from
   // a rounded value. With a K remainder they take the variants that run any K
   // in one launch.
-  constexpr bool kOneLaunchOnly = ElemTraits<E>::Out::kOutBytes == 2;
+  // So do those that end in an epilogue. (Of the others they have no instances of
+  // shapes that only a forced variant reaches.)
+  constexpr bool kEp = has_epilogue<E>();
+  constexpr bool kOneLaunchOnly = ElemTraits<E>::Out::kOutBytes == 2 || kEp;
   int kt_main = kts_per_step > 0 ? (p.K1 / kts_per_step) * kts_per_step : 0;
   if (kOneLaunchOnly && kt_main != p.K1) kt_main = 0;
-  constexpr bool NARROW = (RBC == 2 || RBC == 4) && H == 1 && ElemTraits<E>::Out::kOutBytes == 4;
+  constexpr bool NARROW = (RBC == 2 || RBC == 4) && H == 1 && ElemTraits<E>::Out::kOutBytes == 4 && !kEp;
   if (choice == 1) {
     if constexpr (RBC < 16 && H == 1) {
       // Tile rows of 2, 4 or 8 bytes through the LDS-direct ping-pong pipeline
@@ -1164,9 +1180,11 @@ int launch_class(const Problem& p, int forced, hipStream_t stream, const char** 
       // 4096^3 s8 16x16x2 76 -> 57 us. (f32 keeps its kernels, as below.)
       if (forced == 16 || forced == 17 || (forced == 0 && E != Elem::kF32)) {
         int st = -1;
-        if (forced == 17) {
-          st = launch_variant<E, RBC, 8, 4, 1, 8, 1, 5>(p, 0, p.K1, p.accumulate, stream);
-          if (st == 0) *name = "mmt4d_mfma_128x512_lds_direct";
+        if constexpr (!kEp) {
+          if (forced == 17) {
+            st = launch_variant<E, RBC, 8, 4, 1, 8, 1, 5>(p, 0, p.K1, p.accumulate, stream);
+            if (st == 0) *name = "mmt4d_mfma_128x512_lds_direct";
+          }
         }
         if (st < 0) {
           st = launch_variant<E, RBC, 8, 4, 2, 4, 1, 5>(p, 0, p.K1, p.accumulate, stream);
@@ -1214,9 +1232,11 @@ int launch_class(const Problem& p, int forced, hipStream_t stream, const char** 
       // keeps that pipeline (matrix-pipe bound there: 925 against 959 us).
       constexpr bool kDefault = E != Elem::kF32;
       int st = -1;
-      if (forced == 17) {
-        st = launch_variant<E, RBC, 8, 4, 1, 8, 1, 5>(p, 0, p.K1, p.accumulate, stream);
-        if (st == 0) *name = "mmt4d_mfma_128x512_lds_direct";
+      if constexpr (!kEp) {
+        if (forced == 17) {
+          st = launch_variant<E, RBC, 8, 4, 1, 8, 1, 5>(p, 0, p.K1, p.accumulate, stream);
+          if (st == 0) *name = "mmt4d_mfma_128x512_lds_direct";
+        }
       }
       if (st < 0 && (forced == 16 || forced == 17 || (forced == 0 && kDefault))) {
         st = launch_variant<E, RBC, 8, 4, 2, 4, 1, 5>(p, 0, p.K1, p.accumulate, stream);
@@ -1224,7 +1244,7 @@ int launch_class(const Problem& p, int forced, hipStream_t stream, const char** 
       }
       if (st >= 0) return st;
     }
-    if (kt_main > 0) {
+    if constexpr (!kEp) if (kt_main > 0) {
       int st = -1;
       bool wide = false;
       const int kt_big = E == Elem::kF32 && BIG_PIPE == 3 ? p.K1 : kt_main;  // (runs any K)
@@ -1284,9 +1304,11 @@ int launch_class(const Problem& p, int forced, hipStream_t stream, const char** 
         if (st == 0) *name = "mmt4d_mfma_256x128_lds_direct";
         if (st >= 0) return st;
       }
-      int st = launch_variant<E, RBC, 8, 2, 2, 4, 1, 3>(p, 0, p.K1, p.accumulate, stream);
-      if (st == 0) *name = "mmt4d_mfma_256x128_rhs_direct";
-      if (st >= 0) return st;
+      if constexpr (!kEp) {
+        int st = launch_variant<E, RBC, 8, 2, 2, 4, 1, 3>(p, 0, p.K1, p.accumulate, stream);
+        if (st == 0) *name = "mmt4d_mfma_256x128_rhs_direct";
+        if (st >= 0) return st;
+      }
     }
     choice = 2;
   }
@@ -1401,15 +1423,17 @@ int launch_class(const Problem& p, int forced, hipStream_t stream, const char** 
         if (st > 0) return st;
       }
     }
-    if constexpr (RBC >= 16) {
+    if constexpr (RBC >= 16 && !kEp) {
       int st = launch_variant<E, RBC, 4, 2, 2, 4, 1, 3>(p, 0, p.K1, p.accumulate, stream);
       if (st == 0) *name = "mmt4d_mfma_128x128_rhs_direct";
       if (st >= 0) return st;
     }
-    int st = launch_variant<E, RBC, 4, 4, 2, 2, NKK2, 0>(p, 0, p.K1, p.accumulate, stream);
-    if (st >= 0) { *name = "mmt4d_mfma_128x128"; return st; }
+    if constexpr (!kEp) {
+      int st = launch_variant<E, RBC, 4, 4, 2, 2, NKK2, 0>(p, 0, p.K1, p.accumulate, stream);
+      if (st >= 0) { *name = "mmt4d_mfma_128x128"; return st; }
+    }
   }
-  if constexpr (H == 1) {
+  if constexpr (H == 1 && (!kEp || RBC < 16)) {
     // 64x64 blocks, 8 waves of 32x16, 256 bytes of K per step.
     // Chosen for narrow tile rows when the 64x64 blocks fill the compute units
     // (s8 1024^3 16x16x2: 7.0 -> 6.4 us; with rows of 16 bytes and more the
@@ -1457,8 +1481,10 @@ int launch_class(const Problem& p, int forced, hipStream_t stream, const char** 
   }
   int st = launch_variant<E, RBC, 2, 2, 2, 2, NKK2, 0>(p, 0, p.K1, p.accumulate, stream);
   if (st >= 0) { *name = "mmt4d_mfma_64x64"; return st; }
-  st = launch_variant<E, RBC, 4, 4, 2, 2, NKK2, 0>(p, 0, p.K1, p.accumulate, stream);
-  if (st >= 0) *name = "mmt4d_mfma_128x128";
+  if constexpr (!kEp) {
+    st = launch_variant<E, RBC, 4, 4, 2, 2, NKK2, 0>(p, 0, p.K1, p.accumulate, stream);
+    if (st >= 0) *name = "mmt4d_mfma_128x128";
+  }
   return st;
 }
 

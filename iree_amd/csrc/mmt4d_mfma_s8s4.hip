@@ -9,6 +9,8 @@
 namespace uk_mfma {
 
 int launch_s8(const Problem& p, int forced, hipStream_t stream, const char** name);
+int launch_s8ep_rb8(const Problem& p, int forced, hipStream_t stream, const char** name);
+int launch_s8ep_rb16(const Problem& p, int forced, hipStream_t stream, const char** name);
 }  // namespace uk_mfma
 
 extern "C" int iree_uk_amd_hip_mmt4d_mfma_supported(int32_t M0, int32_t N0, int32_t K0, uint32_t flags);
@@ -57,7 +59,15 @@ constexpr int64_t kExpandFromRows = 512;
 
 }  // namespace
 
-int launch_s8s4(const Problem& p, hipStream_t stream, const char** name) {
+namespace {
+// EPILOGUE: results through an epilogue (Elem::kS8S4Ep; expanded weights: Elem::kS8Ep).
+template <bool EPILOGUE>
+int launch_any_s8s4(const Problem& p, hipStream_t stream, const char** name) {
+  constexpr Elem E = EPILOGUE ? Elem::kS8S4Ep : Elem::kS8S4;
+  auto launch_s8 = [](const Problem& q, int forced, hipStream_t s, const char** n) {
+    if (!EPILOGUE) return uk_mfma::launch_s8(q, forced, s, n);
+    return q.rb >= 16 ? launch_s8ep_rb16(q, 0, s, n) : q.rb == 8 ? launch_s8ep_rb8(q, 0, s, n) : -1;
+  };
   const int64_t rows_m = std::min<int64_t>((int64_t)p.M1 * p.M0, p.out_rows);  // rows that are stored
   const int64_t panel_in_bytes = ((int64_t)p.K1 * p.N0 * p.rb) / 2;
   if (rows_m >= kExpandFromRows && p.N1 > 0 && p.N1 < 65536 && panel_in_bytes % 8 == 0 &&
@@ -112,9 +122,17 @@ int launch_s8s4(const Problem& p, hipStream_t stream, const char** name) {
   }
   if (p.rb < 16) return -1;  // the thin kernel unpacks 16 nibbles per lane: tile rows of 16 and more
   const int64_t cols_n = std::min<int64_t>((int64_t)p.N1 * p.N0, p.out_cols);
-  const int st = rows_m <= 64 ? launch_thin_any<Elem::kS8S4, 16>(p, false, rows_m, cols_n, stream)
-                              : launch_thin_rows<Elem::kS8S4, 16, 4>(p, false, cols_n, stream);
+  const int st = rows_m <= 64 ? launch_thin_any<E, 16>(p, false, rows_m, cols_n, stream)
+                              : launch_thin_rows<E, 16, 4>(p, false, cols_n, stream);
   if (st >= 0) *name = "mmt4d_mfma_thin_s8s4";
   return st;
+}
+}  // namespace
+
+int launch_s8s4(const Problem& p, hipStream_t stream, const char** name) {
+  return launch_any_s8s4<false>(p, stream, name);
+}
+int launch_s8s4ep(const Problem& p, hipStream_t stream, const char** name) {
+  return launch_any_s8s4<true>(p, stream, name);
 }
 }  // namespace uk_mfma

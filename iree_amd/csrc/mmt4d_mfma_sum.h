@@ -33,12 +33,13 @@ struct SumArgs {
   uint32_t dequant;
   const float* row_scale;
   const float* col_scale;
+  Epilogue ep;               // EPILOGUE instances: `out` is the first element of its matrix
 };
 
 // A thread adds four columns of one row: even slices in order, odd slices in order, and
 // those two sums (float errors of 16 slices are then not above those of four waves in
 // eight workgroups: f16 128 x 1024 x 16384 in one order 1.67e-7, here 1.61e-7, there 1.61e-7).
-template <typename Acc, typename Out>
+template <typename Acc, typename Out, bool EPILOGUE = false>
 __global__ __launch_bounds__(kSumThreads)
 void mmt4d_sum_slices_kernel(SumArgs a) {
   constexpr int OB = Out::kOutBytes;
@@ -89,6 +90,21 @@ void mmt4d_sum_slices_kernel(SumArgs a) {
     }
   }
   v += odd;
+  if constexpr (EPILOGUE) {
+    float z[4], rv[4];
+    load_residual(a.ep, row, col, left, rv);
+    const float sm = a.row_scale ? a.row_scale[row] : 1.0f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int c = min(col + e, a.cols - 1);
+      z[e] = (float)v[e] * sm * (a.col_scale ? a.col_scale[c] : 1.0f) + (a.ep.bias ? a.ep.bias[c] : 0.0f);
+    }
+    uk::activate_all(z, a.ep.act);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) z[e] += rv[e];
+    store_row(a.ep, a.out, row, col, left, z);
+    return;
+  }
   if constexpr (OB == 4) {
     if (a.dequant) {
       const float sm = a.row_scale ? a.row_scale[row] : 1.0f;

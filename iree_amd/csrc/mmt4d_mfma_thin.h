@@ -140,7 +140,7 @@ void mmt4d_thin_kernel(Args a) {
   constexpr int HALVES = TT::kHalves;
   constexpr int NCH = 4 * HALVES;             // 16-byte chunks per row per step
   constexpr int KS = NCH * 16;                // bytes of K per row per step
-  constexpr bool S4 = E == Elem::kS8S4;       // 4-bit RHS: half the bytes per row
+  constexpr bool S4 = E == Elem::kS8S4 || E == Elem::kS8S4Ep;       // 4-bit RHS: half the bytes per row
   constexpr int CHAINS = CH > 0 ? CH : thin_chains<E, TM, KSPLIT>();
   static_assert(RBC >= 2, "rows narrower than 2 bytes take the LDS kernels");
   // Rows of 2 and 4 bytes in 16x16 blocks, which are bound by how many loads a unit takes, load
@@ -436,6 +436,30 @@ void mmt4d_thin_kernel(Args a) {
       });
     }
   }
+  // What an epilogue adds, by the kernel's own coordinates: four columns of a row, or with
+  // the operands swapped four rows of a column of the caller's.
+  float rv[has_epilogue<E>() ? OWN : 1][4], bias[has_epilogue<E>() ? OWN : 1][4];
+  if constexpr (has_epilogue<E>()) {
+    for_each_own([&](int i, int tm, int tn) {
+      const int row = row_of(tm), col = first_col(tn);
+      const int left = row < a.out_rows ? a.out_cols - col : 0;
+      if (!a.ep.swapped) {
+        load_residual(a.ep, row, col, left, rv[i]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float one[1];
+          load_residual(a.ep, col + e, row, e < left ? 1 : 0, one);
+          rv[i][e] = one[0];
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int c = a.ep.swapped ? min(row, a.out_rows - 1) : min(col + e, a.out_cols - 1);
+        bias[i][e] = a.ep.bias ? a.ep.bias[max(c, 0)] : 0.0f;
+      }
+    });
+  }
   // The products of a step, whose operands are in registers d, onto chain c.
   auto compute = [&](int d, int c) {
     if constexpr (S4) {
@@ -643,6 +667,31 @@ void mmt4d_thin_kernel(Args a) {
   }
 
   // ---- store --------------------------------------------------------------------
+  if constexpr (has_epilogue<E>()) {
+    for_each_own([&](int i, int tm, int tn) {
+      const int row = row_of(tm), col = first_col(tn);
+      const int left = row < a.out_rows ? a.out_cols - col : 0;
+      if (left <= 0) return;
+      const v4f v = __builtin_convertvector(sum[i], v4f);
+      float z[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        z[e] = (a.col_scale_first ? v[e] * sn[i][e] * sm[i] : v[e] * sm[i] * sn[i][e]) + bias[i][e];
+      uk::activate_all(z, a.ep.act);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) z[e] += rv[i][e];
+      if (!a.ep.swapped) {
+        store_row(a.ep, a.out, row, col, left, z);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float one[1] = {z[e]};
+          store_row(a.ep, a.out, col + e, row, e < left ? 1 : 0, one);
+        }
+      }
+    });
+    return;
+  }
   if constexpr (OB == 4) {
     if (a.dequant) {
       typedef v4f v4f_a4 __attribute__((aligned(4)));

@@ -51,6 +51,21 @@ __device__ __forceinline__ float activate(float x, uint32_t act) {
   }
 }
 
+// The activation of N elements, by one test of the activation for all of them.
+template <int N>
+__device__ __forceinline__ void activate_all(float (&z)[N], uint32_t act) {
+  auto each = [&](auto f) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) z[i] = f(z[i]);
+  };
+  if (act == IREE_UK_AMD_FLAG_ACTIVATION_NONE) return;
+  if (act == IREE_UK_AMD_FLAG_ACTIVATION_SILU) each([](float x) { return activate(x, IREE_UK_AMD_FLAG_ACTIVATION_SILU); });
+  else if (act == IREE_UK_AMD_FLAG_ACTIVATION_GELU_TANH)
+    each([](float x) { return activate(x, IREE_UK_AMD_FLAG_ACTIVATION_GELU_TANH); });
+  else if (act == IREE_UK_AMD_FLAG_ACTIVATION_GELU) each([](float x) { return activate(x, IREE_UK_AMD_FLAG_ACTIVATION_GELU); });
+  else each([](float x) { return activate(x, IREE_UK_AMD_FLAG_ACTIVATION_RELU); });
+}
+
 // f32 to and from the 16-bit floats, rounded to nearest even, subnormals kept.
 struct F32 {
   typedef float T;
