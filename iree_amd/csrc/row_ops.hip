@@ -25,7 +25,8 @@ struct RowArgs {
   char* out;
   float* row_scale;
   int64_t in_stride, second_stride, sum_stride, out_stride;  // bytes
-  int32_t rows, cols, padded_cols, M0, K0;
+  int32_t rows, tiled_rows, cols, padded_cols, M0, K0;   // tiled_rows: M1 * M0
+  int32_t log_waves, rows_a_block, piece;   // rows in registers: waves a row, rows a workgroup, columns next to each other
   uk::FastDiv by_m0, by_k0;
   float epsilon;
   uint32_t act;
@@ -39,8 +40,271 @@ __device__ __forceinline__ uint32_t larger(uint32_t a, float v) {
   return max(a, __float_as_uint(v) & 0x7FFFFFFFu);
 }
 
+// 1 / sqrt(mean + epsilon); an infinite sum is none that a norm can be taken of, and a row
+// without columns has nothing to divide.
+__device__ __forceinline__ float reciprocal_norm(float squares, int cols, float epsilon) {
+  if (cols == 0) return 1.0f;
+  const float mean = squares / (float)cols;
+  return mean < __builtin_inff() ? 1.0f / __builtin_sqrtf(mean + epsilon) : __builtin_nanf("");
+}
+
+// The scale of a row whose largest |u| is `top`, and the factor that takes u to its 8-bit
+// form; 0 for a row that has none.
+template <Form FORM>
+__device__ __forceinline__ void eight_bit_scale(float top, float r, float& scale, float& factor) {
+  constexpr float kLargest = FORM == Form::kS8 ? kLargestS8 : kLargestF8;
+  const float top_y = top * r;
+  factor = 0.0f;
+  if (!(top_y < __builtin_inff())) scale = __builtin_nanf("");
+  else if (top_y < 0x1p-100f || top < 0x1p-110f) scale = 0.0f;
+  else {
+    scale = top_y / kLargest;
+    factor = kLargest / top;
+  }
+}
+
+// ---- rows in registers ---------------------------------------------------------
+//
+// `a.waves` waves a row (a power of two), a lane holding C chunks of 16 columns: a row is
+// read once, its reductions go over the lanes and, through LDS, over the waves, and what is
+// stored comes out of registers. Bound by memory.
+constexpr int kChunk = 16;
+constexpr int kMaxThreads = 1024;
+
+template <typename T, int N>
+struct Any {
+  typedef T V __attribute__((ext_vector_type(N)));
+  typedef V At __attribute__((aligned(sizeof(T))));   // at any address of its elements
+};
+
+// Columns c .. c + 15 of a row of `cols`, zeros beyond its end.
+template <typename IN>
+__device__ __forceinline__ void load_chunk(const char* row, int c, int cols, float (&v)[kChunk]) {
+  using T = typename IN::T;
+  constexpr int N = 16 / sizeof(T);   // 16 bytes a load
+  const T* p = reinterpret_cast<const T*>(row);
+  if (c + kChunk <= cols) {
+#pragma unroll
+    for (int i = 0; i < kChunk; i += N) {
+      const auto x = *reinterpret_cast<const typename Any<T, N>::At*>(p + c + i);
+#pragma unroll
+      for (int e = 0; e < N; ++e) v[i + e] = IN::to_f32(x[e]);
+    }
+  } else {
+    // (No load waits for another: those beyond the row read its last column.)
+#pragma unroll
+    for (int e = 0; e < kChunk; ++e) {
+      const float x = IN::to_f32(p[min(c + e, cols - 1)]);
+      v[e] = c + e < cols ? x : 0.0f;
+    }
+  }
+}
+
+// 16 elements of OB bytes, in words, to the tiles of a row: `at(column)` is where a column
+// goes. Runs of `piece` columns lie next to each other (16, 8, 4, or else single ones).
+template <int OB, typename At>
+__device__ __forceinline__ void store_chunk(const uint32_t (&w)[kChunk * OB / 4], int c, int padded_cols, int piece, At at) {
+  typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+  typedef v4u v4u_any __attribute__((aligned(1)));
+  typedef uint32_t v2u __attribute__((ext_vector_type(2)));
+  typedef v2u v2u_any __attribute__((aligned(1)));
+  typedef uint32_t u32_any __attribute__((aligned(1)));
+  auto store_run = [&](auto columns) __attribute__((always_inline)) {
+    constexpr int P = decltype(columns)::value, WORDS = P * OB / 4;
+#pragma unroll
+    for (int j = 0; j < kChunk; j += P) {
+      if (c + j >= padded_cols) break;
+      char* p = at(c + j);
+      const int first = j * OB / 4;
+      if constexpr (WORDS == 1) *reinterpret_cast<u32_any*>(p) = w[first];
+      else if constexpr (WORDS == 2) *reinterpret_cast<v2u_any*>(p) = v2u{w[first], w[first + 1]};
+      else
+#pragma unroll
+        for (int i = 0; i < WORDS; i += 4)
+          *reinterpret_cast<v4u_any*>(p + 4 * i) = v4u{w[first + i], w[first + i + 1], w[first + i + 2], w[first + i + 3]};
+    }
+  };
+  if (piece == 16) store_run(std::integral_constant<int, 16>{});
+  else if (piece == 8) store_run(std::integral_constant<int, 8>{});
+  else if (piece == 4) store_run(std::integral_constant<int, 4>{});
+  else {
+#pragma unroll
+    for (int j = 0; j < kChunk; ++j) {
+      if (c + j >= padded_cols) break;
+      const uint32_t word = w[j * OB / 4];
+      if constexpr (OB == 1) *at(c + j) = (char)(word >> 8 * (j % 4));
+      else if constexpr (OB == 2) *reinterpret_cast<uint16_t*>(at(c + j)) = (uint16_t)(word >> 16 * (j % 2));
+      else *reinterpret_cast<uint32_t*>(at(c + j)) = word;
+    }
+  }
+}
+
+template <bool NORM, typename IN, Form FORM, int C>
+__global__ __launch_bounds__(kMaxThreads) void row_op_kernel(RowArgs a) {
+  using T = typename IN::T;
+  constexpr int OB = FORM == Form::kSame ? (int)sizeof(T) : 1;
+  __shared__ float part_squares[kMaxThreads / 64];
+  __shared__ uint32_t part_largest[kMaxThreads / 64];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // Consecutive workgroups go to the 8 XCDs in turn, each with an L2 of its own: every XCD
+  // takes a contiguous share of the rows, so that the pieces which neighbouring rows put
+  // into one line of a tile meet in one L2.
+  const uint32_t per_xcd = gridDim.x >> 3;
+  const uint32_t block = blockIdx.x < per_xcd * 8 ? (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3)
+                                                          : blockIdx.x;
+  const int log_waves = a.log_waves, waves = 1 << log_waves;
+  const uint32_t row = block * (uint32_t)a.rows_a_block + (uint32_t)(wave >> log_waves);
+  const bool exists = row < (uint32_t)a.rows, tiled = row < (uint32_t)a.tiled_rows;
+  const int first = ((wave & (waves - 1)) * 64 + lane) * kChunk, step = waves * 64 * kChunk;
+  const uint32_t pm = a.by_m0.div(row), m0 = row - pm * (uint32_t)a.M0;
+  const char* in = a.in + (int64_t)row * a.in_stride;
+  const char* second = a.second + (int64_t)row * a.second_stride;
+  float u[C][kChunk];
+  float squares[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  uint32_t largest = 0;
+#pragma unroll
+  for (int i = 0; i < C; ++i) {
+    const int c = first + i * step;
+#pragma unroll
+    for (int e = 0; e < kChunk; ++e) u[i][e] = 0.0f;
+    if (exists && c < a.cols) {
+      load_chunk<IN>(in, c, a.cols, u[i]);
+      if (a.second) {
+        float s[kChunk];
+        load_chunk<IN>(second, c, a.cols, s);
+        if constexpr (NORM) {
+#pragma unroll
+          for (int e = 0; e < kChunk; ++e) u[i][e] += s[e];
+        } else {
+          uk::activate_all(u[i], a.act);
+#pragma unroll
+          for (int e = 0; e < kChunk; ++e) u[i][e] *= s[e];
+        }
+      } else if constexpr (!NORM) {
+        uk::activate_all(u[i], a.act);
+      }
+    }
+  }
+  if constexpr (NORM) {
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
+      const int c = first + i * step;
+#pragma unroll
+      for (int e = 0; e < kChunk; ++e) squares[e % 4] += u[i][e] * u[i][e];
+      if (a.sum && exists && c < a.cols) {
+        T* sum = reinterpret_cast<T*>(a.sum + (int64_t)row * a.sum_stride) + c;
+        if (c + kChunk <= a.cols) {
+          constexpr int N = 16 / sizeof(T);
+#pragma unroll
+          for (int j = 0; j < kChunk; j += N) {
+            typename Any<T, N>::V x;
+#pragma unroll
+            for (int e = 0; e < N; ++e) x[e] = IN::from_f32(u[i][j + e]);
+            *reinterpret_cast<typename Any<T, N>::At*>(sum + j) = x;
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < kChunk; ++e)
+            if (c + e < a.cols) sum[e] = IN::from_f32(u[i][e]);
+        }
+      }
+      if (a.weight && exists && c < a.cols) {
+        float w[kChunk];
+        load_chunk<IN>(a.weight, c, a.cols, w);
+#pragma unroll
+        for (int e = 0; e < kChunk; ++e) u[i][e] *= w[e];
+      }
+    }
+  }
+  float total = (squares[0] + squares[1]) + (squares[2] + squares[3]);
+  if constexpr (FORM != Form::kSame) {
+#pragma unroll
+    for (int i = 0; i < C; ++i)
+#pragma unroll
+      for (int e = 0; e < kChunk; ++e) largest = larger(largest, u[i][e]);
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    if constexpr (NORM) total += __shfl_xor(total, d);
+    if constexpr (FORM != Form::kSame) largest = max(largest, (uint32_t)__shfl_xor((int)largest, d));
+  }
+  if (waves > 1) {
+    if (lane == 0) {
+      part_squares[wave] = total;
+      part_largest[wave] = largest;
+    }
+    __syncthreads();
+    const int w0 = wave & ~(waves - 1);
+    total = 0.0f;
+    largest = 0;
+    for (int w = 0; w < waves; ++w) {
+      total += part_squares[w0 + w];
+      largest = max(largest, part_largest[w0 + w]);
+    }
+  }
+  if (!tiled) return;
+  float r = 1.0f;
+  if constexpr (NORM) r = reciprocal_norm(total, a.cols, a.epsilon);
+  float factor = r;
+  if constexpr (FORM != Form::kSame) {
+    float scale;
+    eight_bit_scale<FORM>(__uint_as_float(largest), r, scale, factor);
+    if (exists && (threadIdx.x & (waves * 64 - 1)) == 0) a.row_scale[row] = scale;
+    if (factor == 0.0f) {   // (a row without an 8-bit form)
+#pragma unroll
+      for (int i = 0; i < C; ++i)
+#pragma unroll
+        for (int e = 0; e < kChunk; ++e) u[i][e] = 0.0f;
+    }
+  }
+  char* out = a.out + (int64_t)pm * a.out_stride + (int64_t)m0 * a.K0 * OB;
+  auto at = [&](int c) {
+    const uint32_t kt = a.by_k0.div((uint32_t)c);
+    return out + ((int64_t)kt * a.M0 * a.K0 + (c - kt * a.K0)) * OB;
+  };
+#pragma unroll
+  for (int i = 0; i < C; ++i) {
+    const int c = first + i * step;
+    if (c >= a.padded_cols) break;
+    uint32_t w[kChunk * OB / 4];
+#pragma unroll
+    for (int e = 0; e < kChunk; ++e) u[i][e] *= factor;
+    if constexpr (FORM == Form::kS8) {
+      // Adding 1.5 * 2^23 rounds to an integer, whose low bits are the sum's.
+#pragma unroll
+      for (int e = 0; e < kChunk; e += 4) {
+        uint32_t b[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) b[k] = __float_as_uint(u[i][e + k] + 12582912.0f);
+        w[e / 4] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(b[3], b[2], 0x0C0C0400u),
+                                         __builtin_amdgcn_perm(b[1], b[0], 0x0C0C0400u), 0x05040100u);
+      }
+    } else if constexpr (FORM == Form::kF8) {
+#pragma unroll
+      for (int e = 0; e < kChunk; e += 4) {
+        int v = __builtin_amdgcn_cvt_pk_fp8_f32(u[i][e], u[i][e + 1], 0, false);
+        w[e / 4] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(u[i][e + 2], u[i][e + 3], v, true);
+      }
+    } else {
+      constexpr int N = 4 / sizeof(T);
+#pragma unroll
+      for (int e = 0; e < kChunk; e += N) {
+        typename Any<T, N>::V x;
+#pragma unroll
+        for (int k = 0; k < N; ++k) x[k] = IN::from_f32(u[i][e + k]);
+        w[e / N] = __builtin_bit_cast(uint32_t, x);
+      }
+    }
+    store_chunk<OB>(w, c, a.padded_cols, a.piece, at);
+  }
+}
+
+// ---- rows longer than what a workgroup's registers hold ---------------------------
+//
+// One workgroup a row, which it reads twice: for the two sums, and for the output.
 template <bool NORM, typename IN, Form FORM>
-__global__ __launch_bounds__(kThreads) void row_op_kernel(RowArgs a) {
+__global__ __launch_bounds__(kThreads) void row_op_long_kernel(RowArgs a) {
   using T = typename IN::T;
   const uint32_t row = blockIdx.x;
   const uint32_t pm = a.by_m0.div(row), m0 = row - pm * (uint32_t)a.M0;
@@ -95,20 +359,11 @@ __global__ __launch_bounds__(kThreads) void row_op_kernel(RowArgs a) {
     __syncthreads();
   }
   float r = 1.0f;
-  if constexpr (NORM) {
-    const float mean = a.cols ? part_squares[0] / (float)a.cols : 0.0f;
-    // (an infinite sum is none that a norm can be taken of)
-    r = mean < __builtin_inff() ? 1.0f / __builtin_sqrtf(mean + a.epsilon) : __builtin_nanf("");
-    if (!a.cols) r = 1.0f;
-  }
+  if constexpr (NORM) r = reciprocal_norm(part_squares[0], a.cols, a.epsilon);
   float inverse = 0.0f;
   if constexpr (FORM != Form::kSame) {
-    constexpr float kLargest = FORM == Form::kS8 ? kLargestS8 : kLargestF8;
-    const float top = __uint_as_float(part_largest[0]), top_y = top * r;
     float scale;
-    if (!(top_y < __builtin_inff())) scale = __builtin_nanf("");
-    else if (top_y < 0x1p-100f || top < 0x1p-110f) scale = 0.0f;
-    else { scale = top_y / kLargest; inverse = kLargest / top; }
+    eight_bit_scale<FORM>(__uint_as_float(part_largest[0]), r, scale, inverse);
     if (threadIdx.x == 0) a.row_scale[row] = scale;
   }
   for (int c = threadIdx.x; c < a.padded_cols; c += kThreads) {
@@ -161,21 +416,46 @@ extern "C" int iree_uk_amd_hip_launch_row_op(const iree_uk_amd_row_op_t* p, void
   a.by_k0 = uk::FastDiv((uint32_t)p->K0);
   a.epsilon = p->epsilon;
   a.act = p->flags & IREE_UK_AMD_FLAG_ACTIVATION_MASK;
-  const dim3 grid((uint32_t)(p->M1 * p->M0)), block(kThreads);
+  a.tiled_rows = (int32_t)(p->M1 * p->M0);
+  if (p->M0 == 1) {   // (rows as they are: one tile as wide as a row)
+    a.K0 = a.padded_cols;
+    a.by_k0 = uk::FastDiv((uint32_t)a.padded_cols);
+  }
   hipStream_t stream = (hipStream_t)stream_v;
   *kernel_name = p->norm ? "rmsnorm_pack" : "gate_pack";
-  auto go = [&](auto norm, auto in_type) {
+  // Waves a row: as many as leave a lane with one chunk, two where there are rows enough
+  // to fill the chip so, up to 16 waves, where a lane takes up to four.
+  const int64_t chunks = uk::ceil_div(a.padded_cols, kChunk);
+  const int most = a.tiled_rows >= 1024 ? 2 : 1;
+  int log_waves = 0;
+  while (log_waves < 4 && ((int64_t)most << (log_waves + 6)) < chunks) ++log_waves;
+  const int64_t each = uk::ceil_div(chunks, (int64_t)64 << log_waves);
+  const bool in_registers = each <= 4;
+  a.log_waves = log_waves;
+  const int row_threads = 64 << log_waves;
+  const int threads = row_threads < 256 && a.tiled_rows > 1 ? 256 : row_threads;
+  a.rows_a_block = threads / row_threads;
+  a.piece = (int32_t)uk::pow2_divisor(a.K0, 16);
+  auto go = [&](auto norm, auto in_type, auto form_c) {
     constexpr bool N = decltype(norm)::value;
+    constexpr Form F = decltype(form_c)::value;
     using IN = decltype(in_type);
-    auto kernel = form == Form::kS8   ? row_op_kernel<N, IN, Form::kS8>
-                  : form == Form::kF8 ? row_op_kernel<N, IN, Form::kF8>
-                                      : row_op_kernel<N, IN, Form::kSame>;
-    uk::launch(0, kernel, grid, block, 0, stream, a);
+    if (!in_registers) {
+      uk::launch(0, row_op_long_kernel<N, IN, F>, dim3((uint32_t)a.tiled_rows), dim3(kThreads), 0, stream, a);
+      return;
+    }
+    auto kernel = each <= 1 ? row_op_kernel<N, IN, F, 1> : each <= 2 ? row_op_kernel<N, IN, F, 2> : row_op_kernel<N, IN, F, 4>;
+    uk::launch(0, kernel, dim3((uint32_t)uk::ceil_div(a.tiled_rows, a.rows_a_block)), dim3((uint32_t)threads), 0, stream, a);
+  };
+  auto by_form = [&](auto norm, auto in_type) {
+    if (form == Form::kS8) go(norm, in_type, std::integral_constant<Form, Form::kS8>{});
+    else if (form == Form::kF8) go(norm, in_type, std::integral_constant<Form, Form::kF8>{});
+    else go(norm, in_type, std::integral_constant<Form, Form::kSame>{});
   };
   auto by_type = [&](auto norm) {
-    if (in == IREE_UK_AMD_FLAG_IN_TYPE_F32) go(norm, uk::F32{});
-    else if (in == IREE_UK_AMD_FLAG_IN_TYPE_F16) go(norm, uk::F16{});
-    else go(norm, uk::BF16{});
+    if (in == IREE_UK_AMD_FLAG_IN_TYPE_F32) by_form(norm, uk::F32{});
+    else if (in == IREE_UK_AMD_FLAG_IN_TYPE_F16) by_form(norm, uk::F16{});
+    else by_form(norm, uk::BF16{});
   };
   if (p->norm) by_type(std::true_type{});
   else by_type(std::false_type{});
