@@ -65,8 +65,7 @@ __global__ __launch_bounds__(256) void mmt4d_epilogue_kernel(ApartArgs a) {
   uint32_t row, piece;
   a.by_pieces.divmod(id, row, piece);
   const int col = (int)piece * 8, left = a.cols - col;
-  float z[8], rv[8];
-  uk_mfma::load_residual(a.ep, (int)row, col, left, rv);
+  float z[8];
   const char* src = a.z + (int64_t)row * a.z_pitch + (int64_t)col * 4;
   if (left >= 8) {
     const auto v = *reinterpret_cast<const uk_mfma::RowPiece<uk::F32, 8>::Any*>(src);
@@ -78,10 +77,7 @@ __global__ __launch_bounds__(256) void mmt4d_epilogue_kernel(ApartArgs a) {
   }
 #pragma unroll
   for (int e = 0; e < 8; ++e) z[e] += a.ep.bias ? a.ep.bias[min(col + e, a.cols - 1)] : 0.0f;
-  uk::activate_all(z, a.ep.act);
-#pragma unroll
-  for (int e = 0; e < 8; ++e) z[e] += rv[e];
-  uk_mfma::store_row(a.ep, a.out, (int)row, col, left, z);
+  uk_mfma::finish_row(a.ep, a.out, (int)row, col, left, z);
 }
 
 // The most f32 results that wait in the library's buffer for their epilogue: as much as

@@ -37,44 +37,49 @@ __device__ __forceinline__ void by_out_type(const Epilogue& ep, Body&& f) {
 }
 
 // Elements (row, col) .. (row, col + N - 1) of the matrix, of which `left` exist (N and
-// more: all): the residual's elements as f32, zeros where there is none.
-template <int N>
+// more: all): those of the residual (there is one) as f32, zeros where there are none.
+template <typename F, int N>
 __device__ __forceinline__ void load_residual(const Epilogue& ep, int row, int col, int left, float (&v)[N]) {
+  const char* p = ep.residual + (int64_t)row * ep.residual_pitch + (int64_t)col * (int)sizeof(typename F::T);
+  if (left >= N) {
+    const auto x = *reinterpret_cast<const typename RowPiece<F, N>::Any*>(p);
 #pragma unroll
-  for (int e = 0; e < N; ++e) v[e] = 0.0f;
-  if (!ep.residual || left <= 0) return;
-  const char* p = ep.residual + (int64_t)row * ep.residual_pitch + (int64_t)col * ep.out_bytes;
-  by_out_type(ep, [&](auto type) __attribute__((always_inline)) {
-    using F = decltype(type);
-    if (left >= N) {
-      const auto x = *reinterpret_cast<const typename RowPiece<F, N>::Any*>(p);
+    for (int e = 0; e < N; ++e) v[e] = F::to_f32(x[e]);
+  } else {
 #pragma unroll
-      for (int e = 0; e < N; ++e) v[e] = F::to_f32(x[e]);
-    } else {
-#pragma unroll
-      for (int e = 0; e < N; ++e)
-        if (e < left) v[e] = F::to_f32(reinterpret_cast<const typename F::T*>(p)[e]);
-    }
-  });
+    for (int e = 0; e < N; ++e) v[e] = e < left ? F::to_f32(reinterpret_cast<const typename F::T*>(p)[e]) : 0.0f;
+  }
 }
 
 // The same elements, rounded and stored.
-template <int N>
+template <typename F, int N>
 __device__ __forceinline__ void store_row(const Epilogue& ep, char* out, int row, int col, int left, const float (&v)[N]) {
-  if (left <= 0) return;
-  char* p = out + (int64_t)row * ep.out_pitch + (int64_t)col * ep.out_bytes;
+  char* p = out + (int64_t)row * ep.out_pitch + (int64_t)col * (int)sizeof(typename F::T);
+  if (left >= N) {
+    typename RowPiece<F, N>::V x;
+#pragma unroll
+    for (int e = 0; e < N; ++e) x[e] = F::from_f32(v[e]);
+    *reinterpret_cast<typename RowPiece<F, N>::Any*>(p) = x;
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      if (e < left) reinterpret_cast<typename F::T*>(p)[e] = F::from_f32(v[e]);
+  }
+}
+
+// residual + activation(z) of such elements, stored; z has its bias.
+template <int N>
+__device__ __forceinline__ void finish_row(const Epilogue& ep, char* out, int row, int col, int left, float (&z)[N]) {
+  uk::activate_all(z, ep.act);
   by_out_type(ep, [&](auto type) __attribute__((always_inline)) {
     using F = decltype(type);
-    if (left >= N) {
-      typename RowPiece<F, N>::V x;
+    if (ep.residual) {
+      float rv[N];
+      load_residual<F>(ep, row, col, left, rv);
 #pragma unroll
-      for (int e = 0; e < N; ++e) x[e] = F::from_f32(v[e]);
-      *reinterpret_cast<typename RowPiece<F, N>::Any*>(p) = x;
-    } else {
-#pragma unroll
-      for (int e = 0; e < N; ++e)
-        if (e < left) reinterpret_cast<typename F::T*>(p)[e] = F::from_f32(v[e]);
+      for (int e = 0; e < N; ++e) z[e] += rv[e];
     }
+    store_row<F>(ep, out, row, col, left, z);
   });
 }
 

@@ -43,6 +43,7 @@ template <typename Acc, typename Out, bool EPILOGUE = false>
 __global__ __launch_bounds__(kSumThreads)
 void mmt4d_sum_slices_kernel(SumArgs a) {
   constexpr int OB = Out::kOutBytes;
+  if constexpr (EPILOGUE) uk::fetch_arguments<sizeof(SumArgs)>();
   using T = typename std::remove_reference<decltype(Acc{}[0])>::type;
   const int row = blockIdx.y;
   const int col = (blockIdx.x * kSumThreads + threadIdx.x) * 4;
@@ -91,18 +92,14 @@ void mmt4d_sum_slices_kernel(SumArgs a) {
   }
   v += odd;
   if constexpr (EPILOGUE) {
-    float z[4], rv[4];
-    load_residual(a.ep, row, col, left, rv);
+    float z[4];
     const float sm = a.row_scale ? a.row_scale[row] : 1.0f;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int c = min(col + e, a.cols - 1);
       z[e] = (float)v[e] * sm * (a.col_scale ? a.col_scale[c] : 1.0f) + (a.ep.bias ? a.ep.bias[c] : 0.0f);
     }
-    uk::activate_all(z, a.ep.act);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) z[e] += rv[e];
-    store_row(a.ep, a.out, row, col, left, z);
+    finish_row(a.ep, a.out, row, col, left, z);
     return;
   }
   if constexpr (OB == 4) {

@@ -159,6 +159,7 @@ void mmt4d_thin_kernel(Args a) {
   constexpr int NB = TM * TN, OWN = (NB + KSPLIT - 1) / KSPLIT;
   __shared__ v4i partial[KSPLIT][NB][64];
 
+  if constexpr (has_epilogue<E>()) uk::fetch_arguments<sizeof(Args)>();
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t q = lane >> 4, r = lane & 15;
@@ -440,25 +441,38 @@ void mmt4d_thin_kernel(Args a) {
   // the operands swapped four rows of a column of the caller's.
   float rv[has_epilogue<E>() ? OWN : 1][4], bias[has_epilogue<E>() ? OWN : 1][4];
   if constexpr (has_epilogue<E>()) {
-    for_each_own([&](int i, int tm, int tn) {
-      const int row = row_of(tm), col = first_col(tn);
-      const int left = row < a.out_rows ? a.out_cols - col : 0;
-      if (!a.ep.swapped) {
-        load_residual(a.ep, row, col, left, rv[i]);
-      } else {
+#pragma unroll
+    for (int i = 0; i < OWN; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) rv[i][e] = bias[i][e] = 0.0f;
+    if (a.ep.bias) {
+      for_each_own([&](int i, int tm, int tn) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          float one[1];
-          load_residual(a.ep, col + e, row, e < left ? 1 : 0, one);
-          rv[i][e] = one[0];
+          const int c = a.ep.swapped ? min(row_of(tm), a.out_rows - 1) : min(first_col(tn) + e, a.out_cols - 1);
+          bias[i][e] = a.ep.bias[c];
         }
-      }
+      });
+    }
+    if (a.ep.residual) {
+      by_out_type(a.ep, [&](auto type) __attribute__((always_inline)) {
+        using F = decltype(type);
+        for_each_own([&](int i, int tm, int tn) {
+          const int row = row_of(tm), col = first_col(tn);
+          const int left = row < a.out_rows ? a.out_cols - col : 0;
+          if (!a.ep.swapped) {
+            load_residual<F>(a.ep, row, col, left, rv[i]);
+          } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int c = a.ep.swapped ? min(row, a.out_rows - 1) : min(col + e, a.out_cols - 1);
-        bias[i][e] = a.ep.bias ? a.ep.bias[max(c, 0)] : 0.0f;
-      }
-    });
+            for (int e = 0; e < 4; ++e) {
+              float one[1];
+              load_residual<F>(a.ep, col + e, row, e < left ? 1 : 0, one);
+              rv[i][e] = one[0];
+            }
+          }
+        });
+      });
+    }
   }
   // The products of a step, whose operands are in registers d, onto chain c.
   auto compute = [&](int d, int c) {
@@ -668,27 +682,34 @@ void mmt4d_thin_kernel(Args a) {
 
   // ---- store --------------------------------------------------------------------
   if constexpr (has_epilogue<E>()) {
-    for_each_own([&](int i, int tm, int tn) {
-      const int row = row_of(tm), col = first_col(tn);
-      const int left = row < a.out_rows ? a.out_cols - col : 0;
-      if (left <= 0) return;
+    float z[OWN * 4];   // (one array: the activation and the type are looked at once)
+#pragma unroll
+    for (int i = 0; i < OWN; ++i) {
       const v4f v = __builtin_convertvector(sum[i], v4f);
-      float z[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        z[e] = (a.col_scale_first ? v[e] * sn[i][e] * sm[i] : v[e] * sm[i] * sn[i][e]) + bias[i][e];
-      uk::activate_all(z, a.ep.act);
+        z[i * 4 + e] = (a.col_scale_first ? v[e] * sn[i][e] * sm[i] : v[e] * sm[i] * sn[i][e]) + bias[i][e];
+    }
+    uk::activate_all(z, a.ep.act);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) z[e] += rv[i][e];
-      if (!a.ep.swapped) {
-        store_row(a.ep, a.out, row, col, left, z);
-      } else {
+    for (int i = 0; i < OWN; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float one[1] = {z[e]};
-          store_row(a.ep, a.out, col + e, row, e < left ? 1 : 0, one);
+      for (int e = 0; e < 4; ++e) rv[i][e] += z[i * 4 + e];
+    by_out_type(a.ep, [&](auto type) __attribute__((always_inline)) {
+      using F = decltype(type);
+      for_each_own([&](int i, int tm, int tn) {
+        const int row = row_of(tm), col = first_col(tn);
+        const int left = row < a.out_rows ? a.out_cols - col : 0;
+        if (!a.ep.swapped) {
+          store_row<F>(a.ep, a.out, row, col, left, rv[i]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float one[1] = {rv[i][e]};
+            store_row<F>(a.ep, a.out, col + e, row, e < left ? 1 : 0, one);
+          }
         }
-      }
+      });
     });
     return;
   }

@@ -145,6 +145,7 @@ __global__ __launch_bounds__(kMaxThreads) void row_op_kernel(RowArgs a) {
   constexpr int OB = FORM == Form::kSame ? (int)sizeof(T) : 1;
   __shared__ float part_squares[kMaxThreads / 64];
   __shared__ uint32_t part_largest[kMaxThreads / 64];
+  uk::fetch_arguments<sizeof(RowArgs)>();
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // Consecutive workgroups go to the 8 XCDs in turn, each with an L2 of its own: every XCD

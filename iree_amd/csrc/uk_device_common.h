@@ -58,6 +58,19 @@ __device__ __forceinline__ void load_arguments_now(const T& v, const Ts&... vs) 
   load_arguments_now(vs...);
 }
 
+// Has every 64 bytes of a kernel's BYTES of arguments on their way to the scalar cache at
+// once, and waits for them. What the end of a kernel needs then costs no round trip to
+// memory of its own: an argument first touched there took 1.3 us.
+template <int BYTES>
+__device__ __forceinline__ void fetch_arguments() {
+  const auto* p = (const __attribute__((address_space(4))) uint32_t*)__builtin_amdgcn_kernarg_segment_ptr();
+  uint32_t first[(BYTES + 63) / 64];
+#pragma unroll
+  for (int i = 0; i < (BYTES + 63) / 64; ++i) first[i] = p[16 * i];
+#pragma unroll
+  for (int i = 0; i < (BYTES + 63) / 64; ++i) load_arguments_now(first[i]);
+}
+
 // A piece of N bytes (8 or 16) of a matrix row whose end may fall inside or
 // before the piece. `clipped_offset` is where to load it from: the piece's own
 // offset, or the last N bytes of the row where the piece reaches beyond them
