@@ -454,25 +454,6 @@ void mmt4d_thin_kernel(Args a) {
         }
       });
     }
-    if (a.ep.residual) {
-      by_out_type(a.ep, [&](auto type) __attribute__((always_inline)) {
-        using F = decltype(type);
-        for_each_own([&](int i, int tm, int tn) {
-          const int row = row_of(tm), col = first_col(tn);
-          const int left = row < a.out_rows ? a.out_cols - col : 0;
-          if (!a.ep.swapped) {
-            load_residual<F>(a.ep, row, col, left, rv[i]);
-          } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              float one[1];
-              load_residual<F>(a.ep, col + e, row, e < left ? 1 : 0, one);
-              rv[i][e] = one[0];
-            }
-          }
-        });
-      });
-    }
   }
   // The products of a step, whose operands are in registers d, onto chain c.
   auto compute = [&](int d, int c) {
@@ -564,6 +545,27 @@ void mmt4d_thin_kernel(Args a) {
       }
       i += U;
     } while (i + U + D <= my_steps);
+  }
+  if constexpr (has_epilogue<E>()) {
+    if (a.ep.residual) {
+      by_out_type(a.ep, [&](auto type) __attribute__((always_inline)) {
+        using F = decltype(type);
+        for_each_own([&](int i, int tm, int tn) {
+          const int row = row_of(tm), col = first_col(tn);
+          const int left = row < a.out_rows ? a.out_cols - col : 0;
+          if (!a.ep.swapped) {
+            load_residual<F>(a.ep, row, col, left, rv[i]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              float one[1];
+              load_residual<F>(a.ep, col + e, row, e < left ? 1 : 0, one);
+              rv[i][e] = one[0];
+            }
+          }
+        });
+      });
+    }
   }
   // The products of the last steps: a chain's sum is read, to be added up or copied, soon
   // after them, and the compiler counts the instructions that have to lie in between
