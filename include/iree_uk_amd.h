@@ -885,9 +885,10 @@ IREE_UK_AMD_EXPORT void iree_uk_amd_gate_pack_p(
  *   z[i][j] = (float)(sum_k lhs[i][k] * rhs[j][k]) * row_scale[i] * col_scale[j]
  *   out[i][j] = residual[i][j] + activation(z[i][j] + bias[j])
  *
- * evaluated in f32 from left to right and rounded once, at the end. row_scale,
- * bias, col_scale: out_size0 / out_size1 f32 entries; any of them may be NULL
- * and then reads as 1, 0 and 1. residual_buffer: a matrix of the out type with
+ * evaluated in f32 from left to right (the sum with the bias and the product
+ * with col_scale with or without a rounding in between) and rounded to the out
+ * type once, at the end. row_scale, col_scale, bias: out_size0, out_size1
+ * and out_size1 f32 entries; any of them may be NULL and then reads as 1, 1 and 0. residual_buffer: a matrix of the out type with
  * a stride of its own, or NULL; it may be the output itself (same offset and
  * stride), else the two do not overlap. Operand arguments, tile sizes and
  * `flags` are those of iree_uk_mmt4d for a type with a 32-bit accumulator,

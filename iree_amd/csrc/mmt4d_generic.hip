@@ -95,13 +95,13 @@ __global__ __launch_bounds__(kThreads) void mmt4d_generic_kernel(Mmt4dArgs a) {
     };
     // The dequantizing store, with what follows the scales of a linear layer.
     auto store_scaled = [&](float acc) {
-      float v = scaled(acc);
       if (!a.epilogue) {
-        reinterpret_cast<float*>(a.out)[o] = v;
+        reinterpret_cast<float*>(a.out)[o] = scaled(acc);
         return;
       }
-      if (a.bias) v += a.bias[j * N0 + j0];
-      v = uk::activate(v, a.act);
+      const float rs = a.row_scale ? a.row_scale[i * M0 + i0] : 1.0f;
+      const float cs = a.col_scale ? a.col_scale[j * N0 + j0] : 1.0f;
+      float v = uk::activate(__builtin_fmaf(acc * rs, cs, a.bias ? a.bias[j * N0 + j0] : 0.0f), a.act);
       const int64_t ro = (i * M0 + i0) * a.residual_stride + j * N0 + j0;
       auto store = [&](auto type) {
         using F = decltype(type);

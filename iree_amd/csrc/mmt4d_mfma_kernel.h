@@ -279,6 +279,21 @@ __device__ __forceinline__ void static_for(F&& f) {
   }
 }
 
+// Loads from a buffer resource (its base, the same in all lanes), a lane's bytes and a
+// scalar's: a lane's address is one register that the K loop never touches, where an
+// address of its own takes a vector addition for every load, in the pipe that the f32
+// matrix instructions keep busy (f32 16x16x1 in 32x32 blocks: 515 x 1027 x 769 17.0 ->
+// 15.0 us, 700 x 700 x 3000 41.0 -> 34.6, 1500 x 1500 x 1000 52.6 -> 44.9). What lies
+// kBeyond in a lane is outside the resource: such a load returns zeros and reads nothing.
+constexpr uint32_t kBeyond = 0x80000000u;
+struct Operand {
+  __amdgpu_buffer_rsrc_t buffer;
+  const char* base;
+};
+__device__ __forceinline__ Operand operand_at(const char* base) {
+  return {__builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, (int)kBeyond, 0x00027000), base};
+}
+
 // What PIPE 5 loads in place of K-tiles beyond K.
 static __device__ __attribute__((aligned(16))) const uint32_t kZeroPiece[4] = {0, 0, 0, 0};
 
@@ -1684,7 +1699,7 @@ void mmt4d_mfma_kernel(Args a) {
       };
       // (256x256 blocks that end in an epilogue, too: unrolled they came out with 122
       // registers in scratch memory, as the blocks of the other types and without an
-      // epilogue do not; f8 2048 x 8192 x 28672 1627 us, so 0.)
+      // epilogue do not; f8 2048 x 8192 x 28672 1627 us, so 310.)
       if constexpr ((TAIL || (has_epilogue<E>() && TM * TN >= 32)) && !S16) {
         // Rolled: the test of every load against the end of K, in every copy of
         // the unrolled loop, asked for more registers than there are (f8 4096 x
@@ -1841,63 +1856,12 @@ void mmt4d_mfma_kernel(Args a) {
       sn[e] = a.col_scale ? a.col_scale[c] : 1.0f;
       bias[e] = a.ep.bias ? a.ep.bias[c] : 0.0f;
     }
-    // Residual and row scale of the rounds ahead, as many as keep memory busy (one round at a
-    // time waited for each: s8 2048 x 14336 x 4096 with a residual 132 us, without 108).
-    constexpr int ROUNDS = ROWS / RPI, AHEAD = ROUNDS < 4 ? ROUNDS : 4;
-    static_assert(ROUNDS % AHEAD == 0, "whole turns");
-    typedef uint32_t v4u_any __attribute__((ext_vector_type(4), aligned(2)));
-    uint32_t ahead[AHEAD][8];   // (16-bit types: four words of eight)
-    float scale_ahead[AHEAD];
-    const bool f32 = a.ep.out_type == IREE_UK_AMD_FLAG_OUT_TYPE_F32;
-    auto row_at = [&](int pass, int round) { return (wm * TM + pass * PASS) * 16 + round * RPI + row0; };
-    auto fetch = [&](int pass, int round, int slot) __attribute__((always_inline)) {
-      const int row = min(row_at(pass, round), rows_here - 1) + row_origin;   // (beyond: not stored)
-      scale_ahead[slot] = a.row_scale ? a.row_scale[row] : 1.0f;
-      if (!a.ep.residual || left < 8) return;   // (the end of a row is read where it is stored)
-      const char* p = a.ep.residual + (int64_t)row * a.ep.residual_pitch + (int64_t)(col_origin + col) * a.ep.out_bytes;
-      const v4u_any x = *reinterpret_cast<const v4u_any*>(p);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) ahead[slot][i] = x[i];
-      if (f32) {
-        const v4u_any y = *reinterpret_cast<const v4u_any*>(p + 16);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) ahead[slot][4 + i] = y[i];
-      }
-    };
-    auto finish = [&](int pass, int round, int slot) __attribute__((always_inline)) {
-      const int row = round * RPI + row0, block_row = row_at(pass, round);
-      if (block_row >= rows_here || left <= 0) return;
-      const int mrow = row_origin + block_row, mcol = col_origin + col;
-      const uint32_t turn = (uint32_t)row & (CH - 1);
-      const v4f lo = mine[row * CH + ((2 * c8) ^ turn)], hi = mine[row * CH + ((2 * c8 + 1) ^ turn)];
-      float z[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) z[e] = (e < 4 ? lo[e] : hi[e - 4]) * scale_ahead[slot] * sn[e] + bias[e];
-      if (left < 8) {
-        finish_row(a.ep, a.out, mrow, mcol, left, z);
-        return;
-      }
-      uk::activate_all(z, a.ep.act);
-      by_out_type(a.ep, [&](auto type) __attribute__((always_inline)) {
-        using F = decltype(type);
-        if (a.ep.residual) {
-          constexpr int N = 4 / sizeof(typename F::T);
-#pragma unroll
-          for (int i = 0; i < 8; i += N) {
-            const auto x = __builtin_bit_cast(typename RowPiece<F, N>::V, ahead[slot][i / N]);
-#pragma unroll
-            for (int e = 0; e < N; ++e) z[i + e] += F::to_f32(x[e]);
-          }
-        }
-        store_row<F>(a.ep, a.out, mrow, mcol, left, z);
-      });
-    };
     if (rows_here <= 0) return;
-#pragma unroll
-    for (int pass = 0; pass < TM / PASS; ++pass) {
-#pragma unroll
-      for (int k = 0; k < AHEAD; ++k) fetch(pass, k, k);
-      if (pass == 0) __syncthreads();   // (every operand has been read, every LDS-direct load has landed)
+    constexpr int ROUNDS = ROWS / RPI, PASSES = TM / PASS;
+    const int wave_row = wm * TM * 16;
+    auto put_sums = [&](int pass) __attribute__((always_inline)) {
+      // (Before the first: every operand has been read, every LDS-direct load has landed.)
+      if (pass == 0) __syncthreads();
 #pragma unroll
       for (int t = 0; t < PASS; ++t)
 #pragma unroll
@@ -1907,16 +1871,123 @@ void mmt4d_mfma_kernel(Args a) {
               __builtin_convertvector(acc[pass * PASS + t][tn], v4f);
         }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    };
+    auto scaled_row = [&](int row, float sm, float (&z)[8]) __attribute__((always_inline)) {
+      const uint32_t turn = (uint32_t)row & (CH - 1);
+      const v4f lo = mine[row * CH + ((2 * c8) ^ turn)], hi = mine[row * CH + ((2 * c8 + 1) ^ turn)];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) z[e] = __builtin_fmaf((e < 4 ? lo[e] : hi[e - 4]) * sm, sn[e], bias[e]);
+    };
+    if (__any(left > 0 && left < 8)) {
+      // The matrix, or the workgroup's share of it, ends inside eight columns.
+#pragma unroll
+      for (int pass = 0; pass < PASSES; ++pass) {
+        put_sums(pass);
 #pragma nounroll
-      for (int i = 0; i < ROUNDS; i += AHEAD) {
+        for (int i = 0; i < ROWS; i += RPI) {
+          const int block_row = wave_row + pass * ROWS + i + row0;
+          if (block_row < rows_here && left > 0) {
+            float z[8];
+            scaled_row(i + row0, a.row_scale ? a.row_scale[row_origin + block_row] : 1.0f, z);
+            finish_row(a.ep, a.out, row_origin + block_row, col_origin + col, left, z);
+          }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      }
+      return;
+    }
+    // Else no lane branches: what it has no row or column for is outside a buffer resource,
+    // its loads give zeros and its stores are dropped. The compiler then knows how many loads
+    // and stores lie between the load of a residual row and its use, AHEAD rounds later,
+    // and waits for that one alone. (With a branch around each it waited for everything in
+    // flight, the last round's stores included: s8 4096^3 with GELU and a residual 73 us, so 66.)
+    const Operand to = operand_at(a.out + (int64_t)row_origin * a.ep.out_pitch + (int64_t)col_origin * a.ep.out_bytes);
+    const Operand from = operand_at(a.ep.residual + (int64_t)row_origin * a.ep.residual_pitch +
+                                    (int64_t)col_origin * a.ep.out_bytes);
+    const Operand scales = operand_at(reinterpret_cast<const char*>(a.row_scale + row_origin));
+    const uint32_t out_pitch = (uint32_t)a.ep.out_pitch, residual_pitch = (uint32_t)a.ep.residual_pitch;
+    const uint32_t first_row = (uint32_t)(wave_row + row0);   // the lane's
+    const uint32_t out_lane = first_row * out_pitch + (uint32_t)col * a.ep.out_bytes;
+    const uint32_t residual_lane = a.ep.residual ? first_row * residual_pitch + (uint32_t)col * a.ep.out_bytes : kBeyond;
+    const uint32_t scale_lane = a.row_scale ? first_row * 4 : kBeyond;
+    const int lane_rows = left > 0 ? min(rows_here - wave_row, TM * 16) - row0 : 0;   // rows from the first on
+    const bool bf16 = a.ep.out_type == IREE_UK_AMD_FLAG_OUT_TYPE_BF16, scaled = a.row_scale != nullptr;
+    auto rounds = [&](auto pieces) __attribute__((always_inline)) {
+      // 16-byte pieces of eight columns, and 64 bytes of a lane ahead (with 128 of f32 the 256x256
+      // blocks had registers in scratch memory, f8 in its K loop: 684 us).
+      constexpr int PIECES = decltype(pieces)::value, MOST = 4 / PIECES, AHEAD = ROUNDS < MOST ? ROUNDS : MOST;
+      static_assert(ROUNDS % AHEAD == 0, "whole turns");
+      v4i ahead[AHEAD][PIECES];
+      float sm[AHEAD];
+      auto fetch = [&](int round, int slot) __attribute__((always_inline)) {
+        const bool ok = round * RPI < lane_rows;
+#pragma unroll
+        for (int h = 0; h < PIECES; ++h)
+          ahead[slot][h] = __builtin_bit_cast(
+              v4i, __builtin_amdgcn_raw_buffer_load_b128(from.buffer, (ok ? residual_lane : kBeyond) + 16 * h,
+                                                         (uint32_t)(round * RPI) * residual_pitch, 0));
+        const float x = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(
+                                                      scales.buffer, ok ? scale_lane : kBeyond, (uint32_t)(round * RPI) * 4, 0));
+        sm[slot] = scaled ? x : 1.0f;
+      };
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) fetch(k, k);
+#pragma nounroll
+      for (int round0 = 0; round0 < PASSES * ROUNDS; round0 += AHEAD) {
+#pragma unroll
+        for (int pass = 0; pass < PASSES; ++pass)
+          if (round0 == pass * ROUNDS) put_sums(pass);
 #pragma unroll
         for (int k = 0; k < AHEAD; ++k) {
-          finish(pass, i + k, k);
-          if (i + k + AHEAD < ROUNDS) fetch(pass, i + k + AHEAD, k);
+          const int round = round0 + k;
+          float z[8];
+          scaled_row((round & (ROUNDS - 1)) * RPI + row0, sm[k], z);
+          uk::activate_all(z, a.ep.act);
+#pragma unroll
+          for (int h = 0; h < PIECES; ++h) {
+            const v4i x = ahead[k][h];
+            if constexpr (PIECES == 2) {
+              const v4f y = __builtin_bit_cast(v4f, x);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) z[4 * h + e] += y[e];
+            } else if (bf16) {
+              const auto y = __builtin_bit_cast(RowPiece<uk::BF16, 8>::V, x);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) z[e] += uk::BF16::to_f32(y[e]);
+            } else {
+              const auto y = __builtin_bit_cast(RowPiece<uk::F16, 8>::V, x);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) z[e] += uk::F16::to_f32(y[e]);
+            }
+          }
+          fetch(round + AHEAD, k);
+          const uint32_t at = round * RPI < lane_rows ? out_lane : kBeyond;
+#pragma unroll
+          for (int h = 0; h < PIECES; ++h) {
+            v4i x;
+            if constexpr (PIECES == 2) {
+              x = __builtin_bit_cast(v4i, v4f{z[4 * h], z[4 * h + 1], z[4 * h + 2], z[4 * h + 3]});
+            } else if (bf16) {
+              RowPiece<uk::BF16, 8>::V y;
+#pragma unroll
+              for (int e = 0; e < 8; ++e) y[e] = uk::BF16::from_f32(z[e]);
+              x = __builtin_bit_cast(v4i, y);
+            } else {
+              RowPiece<uk::F16, 8>::V y;
+#pragma unroll
+              for (int e = 0; e < 8; ++e) y[e] = uk::F16::from_f32(z[e]);
+              x = __builtin_bit_cast(v4i, y);
+            }
+            __builtin_amdgcn_raw_buffer_store_b128(x, to.buffer, at + 16 * h, (uint32_t)(round * RPI) * out_pitch, 0);
+          }
         }
+        // (the next pass's sums take the place of what has been read)
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       }
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    }
+    };
+    static_assert((ROUNDS & (ROUNDS - 1)) == 0, "a power of two");
+    if (a.ep.out_type == IREE_UK_AMD_FLAG_OUT_TYPE_F32) rounds(std::integral_constant<int, 2>{});
+    else rounds(std::integral_constant<int, 1>{});
     return;
   }
   if constexpr (OB == 4) {

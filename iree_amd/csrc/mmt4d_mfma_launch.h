@@ -153,6 +153,7 @@ int launch_variant(const Problem& p, int kt_begin, int kt_count, bool accumulate
       span_a >= (1ll << 31)) {
     return -1;
   }
+  if (has_epilogue<E>() && p.ep.residual && (int64_t)SH::BM * p.ep.residual_pitch + SH::BN * 4 >= (1ll << 31)) return -1;
   set_divisors(a);
   auto go = [&](auto tail_c) {
     auto kernel = mmt4d_mfma_kernel<E, RBC, TM, TN, WGM, WGN, NKK, PIPE, decltype(tail_c)::value, SLICED>;

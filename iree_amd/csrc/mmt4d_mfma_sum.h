@@ -97,7 +97,7 @@ void mmt4d_sum_slices_kernel(SumArgs a) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int c = min(col + e, a.cols - 1);
-      z[e] = (float)v[e] * sm * (a.col_scale ? a.col_scale[c] : 1.0f) + (a.ep.bias ? a.ep.bias[c] : 0.0f);
+      z[e] = __builtin_fmaf((float)v[e] * sm, a.col_scale ? a.col_scale[c] : 1.0f, a.ep.bias ? a.ep.bias[c] : 0.0f);
     }
     finish_row(a.ep, a.out, row, col, left, z);
     return;

@@ -53,21 +53,8 @@ namespace uk_mfma {
 
 typedef int v2i __attribute__((ext_vector_type(2)));
 
-// Loads from a buffer resource (its base, the same in all lanes), a lane's bytes and a
-// scalar's: a lane's address is one register that the K loop never touches, where an
-// address of its own takes a vector addition for every load, in the pipe that the f32
-// matrix instructions keep busy (f32 16x16x1 in 32x32 blocks: 515 x 1027 x 769 17.0 ->
-// 15.0 us, 700 x 700 x 3000 41.0 -> 34.6, 1500 x 1500 x 1000 52.6 -> 44.9). What lies
-// kBeyond in a lane is outside the resource: such a load returns zeros and reads nothing.
-// NT: non-temporal.
-constexpr uint32_t kBeyond = 0x80000000u;
-struct Operand {
-  __amdgpu_buffer_rsrc_t buffer;
-  const char* base;
-};
-__device__ __forceinline__ Operand operand_at(const char* base) {
-  return {__builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, (int)kBeyond, 0x00027000), base};
-}
+// (Loads through buffer resources: Operand and kBeyond of mmt4d_mfma_kernel.h.) NT:
+// non-temporal.
 template <bool NT>
 __device__ __forceinline__ v4i load16(const Operand& from, uint32_t lane_bytes, uint32_t bytes) {
   return __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(from.buffer, lane_bytes, bytes, NT ? 2 : 0));
@@ -690,7 +677,8 @@ void mmt4d_thin_kernel(Args a) {
       const v4f v = __builtin_convertvector(sum[i], v4f);
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        z[i * 4 + e] = (a.col_scale_first ? v[e] * sn[i][e] * sm[i] : v[e] * sm[i] * sn[i][e]) + bias[i][e];
+        z[i * 4 + e] = a.col_scale_first ? __builtin_fmaf(v[e] * sn[i][e], sm[i], bias[i][e])
+                                         : __builtin_fmaf(v[e] * sm[i], sn[i][e], bias[i][e]);
     }
     uk::activate_all(z, a.ep.act);
 #pragma unroll

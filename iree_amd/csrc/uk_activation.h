@@ -24,17 +24,16 @@ __device__ __forceinline__ float times_sigmoid(float x, float t) {
 // to 1.5e-7 for z >= 0): x - x erfc(z) / 2 for positive x, x erfc(z) / 2 for negative,
 // so nothing cancels in the negative tail.
 __device__ __forceinline__ float gelu(float x) {
-  const float ax = __builtin_fabsf(x);
+  // (From 64 on the tail is zero, an infinite x, whose tail would be infinity times zero, among them.)
+  const float ax = __builtin_fminf(__builtin_fabsf(x), 64.0f);
   const float z = ax * 0.70710678f;
   const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f, z, 1.0f));
   float p = __builtin_fmaf(1.061405429f, t, -1.453152027f);
   p = __builtin_fmaf(p, t, 1.421413741f);
   p = __builtin_fmaf(p, t, -0.284496736f);
   p = __builtin_fmaf(p, t, 0.254829592f);
-  // (An infinite x has a tail of infinity times zero; its limit is zero.)
-  const float e = __builtin_amdgcn_exp2f(-1.44269504f * z * z);
-  const float tail = e == 0.0f ? 0.0f : 0.5f * ax * (p * t * e);
-  return x > 0.0f ? x - tail : x < 0.0f ? -tail : x;
+  const float tail = 0.5f * ax * (p * t * __builtin_amdgcn_exp2f(-1.44269504f * z * z));
+  return (x < 0.0f ? 0.0f : x) - tail;   // (a NaN is not below zero, and stays)
 }
 
 // `act` is an IREE_UK_AMD_FLAG_ACTIVATION_* value, the same in all lanes. The comparison of

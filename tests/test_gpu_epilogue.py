@@ -177,6 +177,7 @@ def test_epilogue_in_a_captured_graph(gpu):
                 g.replay()
                 torch.cuda.synchronize()
             call()
+            torch.cuda.synchronize()   # (the replay runs on another stream, and writes the same matrix)
             g.replay()
             torch.cuda.synchronize()
         finally:
