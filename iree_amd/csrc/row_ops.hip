@@ -77,28 +77,43 @@ struct Any {
   typedef V At __attribute__((aligned(sizeof(T))));   // at any address of its elements
 };
 
-// Columns c .. c + 15 of a row of `cols`, zeros beyond its end.
+// Columns c .. c + 15 of a row as they lie in memory. Loading and using them are two steps,
+// and no lane branches in the first: what a kernel loads is then in flight together, one
+// round trip to memory where `load, convert` for each of residual and weight made three.
 template <typename IN>
-__device__ __forceinline__ void load_chunk(const char* row, int c, int cols, float (&v)[kChunk]) {
+struct Chunk {
   using T = typename IN::T;
-  constexpr int N = 16 / sizeof(T);   // 16 bytes a load
-  const T* p = reinterpret_cast<const T*>(row);
-  if (c + kChunk <= cols) {
+  static constexpr int PIECES = (int)sizeof(T), N = kChunk / PIECES;   // of 16 bytes; columns of one
+  uint32_t w[PIECES][4];
+
+  // `row_bytes` > 0: of the row. A piece beyond its end is loaded from its last 16 bytes.
+  __device__ __forceinline__ void load(const char* row, int c, uint32_t row_bytes) {
+    typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+    typedef v4u v4u_any __attribute__((aligned(1)));
+    const uint32_t off = (uint32_t)c * (uint32_t)sizeof(T);
 #pragma unroll
-    for (int i = 0; i < kChunk; i += N) {
-      const auto x = *reinterpret_cast<const typename Any<T, N>::At*>(p + c + i);
+    for (int p = 0; p < PIECES; ++p) {
+      if (row_bytes >= 16) {   // (the same in all lanes)
+        const v4u x = *reinterpret_cast<const v4u_any*>(row + uk::clipped_offset<16>(off + 16 * p, row_bytes));
 #pragma unroll
-      for (int e = 0; e < N; ++e) v[i + e] = IN::to_f32(x[e]);
-    }
-  } else {
-    // (No load waits for another: those beyond the row read its last column.)
-#pragma unroll
-    for (int e = 0; e < kChunk; ++e) {
-      const float x = IN::to_f32(p[min(c + e, cols - 1)]);
-      v[e] = c + e < cols ? x : 0.0f;
+        for (int i = 0; i < 4; ++i) w[p][i] = x[i];
+      } else {
+        uk::load_short_row<16>(w[p], row, off + 16 * p == 0 ? (int32_t)row_bytes : 0, 0);
+      }
     }
   }
-}
+  // Those columns as f32, zeros beyond the row.
+  __device__ __forceinline__ void values(int c, uint32_t row_bytes, float (&v)[kChunk]) {
+    const uint32_t off = (uint32_t)c * (uint32_t)sizeof(T);
+#pragma unroll
+    for (int p = 0; p < PIECES; ++p) {
+      if (row_bytes >= 16) uk::clip_piece<16>(w[p], uk::row_bytes_left(row_bytes, off + 16 * p), 0);
+      const auto x = __builtin_bit_cast(typename Any<T, N>::V, w[p]);
+#pragma unroll
+      for (int e = 0; e < N; ++e) v[p * N + e] = IN::to_f32(x[e]);
+    }
+  }
+};
 
 // 16 elements of OB bytes, in words, to the tiles of a row: `at(column)` is where a column
 // goes. Runs of `piece` columns lie next to each other (16, 8, 4, or else single ones).
@@ -164,59 +179,68 @@ __global__ __launch_bounds__(kMaxThreads) void row_op_kernel(RowArgs a) {
   float u[C][kChunk];
   float squares[4] = {0.0f, 0.0f, 0.0f, 0.0f};
   uint32_t largest = 0;
-#pragma unroll
-  for (int i = 0; i < C; ++i) {
-    const int c = first + i * step;
-#pragma unroll
-    for (int e = 0; e < kChunk; ++e) u[i][e] = 0.0f;
-    if (exists && c < a.cols) {
-      load_chunk<IN>(in, c, a.cols, u[i]);
-      if (a.second) {
-        float s[kChunk];
-        load_chunk<IN>(second, c, a.cols, s);
-        if constexpr (NORM) {
-#pragma unroll
-          for (int e = 0; e < kChunk; ++e) u[i][e] += s[e];
-        } else {
-          uk::activate_all(u[i], a.act);
-#pragma unroll
-          for (int e = 0; e < kChunk; ++e) u[i][e] *= s[e];
-        }
-      } else if constexpr (!NORM) {
-        uk::activate_all(u[i], a.act);
-      }
-    }
-  }
-  if constexpr (NORM) {
+  const uint32_t row_bytes = (uint32_t)a.cols * (uint32_t)sizeof(T);
+  if (exists && a.cols > 0) {   // (the same in all lanes of a wave)
+    // (Four chunks, of gates only, one after the other: their registers.)
+    constexpr int P = C <= 2 ? C : 1;
+    Chunk<IN> x[P], y[P], z[NORM ? P : 1];
 #pragma unroll
     for (int i = 0; i < C; ++i) {
-      const int c = first + i * step;
+      const int c = first + i * step, k = i % P;
+      if (k == 0) {
 #pragma unroll
-      for (int e = 0; e < kChunk; ++e) squares[e % 4] += u[i][e] * u[i][e];
-      if (a.sum && exists && c < a.cols) {
-        T* sum = reinterpret_cast<T*>(a.sum + (int64_t)row * a.sum_stride) + c;
-        if (c + kChunk <= a.cols) {
-          constexpr int N = 16 / sizeof(T);
-#pragma unroll
-          for (int j = 0; j < kChunk; j += N) {
-            typename Any<T, N>::V x;
-#pragma unroll
-            for (int e = 0; e < N; ++e) x[e] = IN::from_f32(u[i][j + e]);
-            *reinterpret_cast<typename Any<T, N>::At*>(sum + j) = x;
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < kChunk; ++e)
-            if (c + e < a.cols) sum[e] = IN::from_f32(u[i][e]);
+        for (int j = 0; j < P; ++j) {
+          x[j].load(in, c + j * step, row_bytes);
+          if (a.second) y[j].load(second, c + j * step, row_bytes);
+          if (NORM && a.weight) z[j].load(a.weight, c + j * step, row_bytes);
         }
       }
-      if (a.weight && exists && c < a.cols) {
-        float w[kChunk];
-        load_chunk<IN>(a.weight, c, a.cols, w);
+      float v[kChunk];
+      x[k].values(c, row_bytes, u[i]);
+      if constexpr (NORM) {
+        if (a.second) {
+          y[k].values(c, row_bytes, v);
 #pragma unroll
-        for (int e = 0; e < kChunk; ++e) u[i][e] *= w[e];
+          for (int e = 0; e < kChunk; ++e) u[i][e] += v[e];
+        }
+#pragma unroll
+        for (int e = 0; e < kChunk; ++e) squares[e % 4] += u[i][e] * u[i][e];
+        if (a.sum && c < a.cols) {
+          T* sum = reinterpret_cast<T*>(a.sum + (int64_t)row * a.sum_stride) + c;
+          if (c + kChunk <= a.cols) {
+            constexpr int N = 16 / sizeof(T);
+#pragma unroll
+            for (int j = 0; j < kChunk; j += N) {
+              typename Any<T, N>::V h;
+#pragma unroll
+              for (int e = 0; e < N; ++e) h[e] = IN::from_f32(u[i][j + e]);
+              *reinterpret_cast<typename Any<T, N>::At*>(sum + j) = h;
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < kChunk; ++e)
+              if (c + e < a.cols) sum[e] = IN::from_f32(u[i][e]);
+          }
+        }
+        if (a.weight) {
+          z[k].values(c, row_bytes, v);
+#pragma unroll
+          for (int e = 0; e < kChunk; ++e) u[i][e] *= v[e];
+        }
+      } else {
+        uk::activate_all<true>(u[i], a.act);
+        if (a.second) {
+          y[k].values(c, row_bytes, v);
+#pragma unroll
+          for (int e = 0; e < kChunk; ++e) u[i][e] *= v[e];
+        }
       }
     }
+  } else {
+#pragma unroll
+    for (int i = 0; i < C; ++i)
+#pragma unroll
+      for (int e = 0; e < kChunk; ++e) u[i][e] = 0.0f;
   }
   float total = (squares[0] + squares[1]) + (squares[2] + squares[3]);
   if constexpr (FORM != Form::kSame) {
@@ -337,7 +361,7 @@ __global__ __launch_bounds__(kThreads) void row_op_long_kernel(RowArgs a) {
   };
   auto u_of = [&](int c, float h) {
     if constexpr (NORM) return a.weight ? h * IN::to_f32(weight[c]) : h;
-    float v = uk::activate(h, a.act);
+    float v = uk::activate<true>(h, a.act);
     return a.second ? v * IN::to_f32(second[c]) : v;
   };
   __shared__ float part_squares[kThreads];
@@ -424,14 +448,19 @@ extern "C" int iree_uk_amd_hip_launch_row_op(const iree_uk_amd_row_op_t* p, void
   }
   hipStream_t stream = (hipStream_t)stream_v;
   *kernel_name = p->norm ? "rmsnorm_pack" : "gate_pack";
-  // Waves a row: as many as leave a lane with one chunk, two where there are rows enough
-  // to fill the chip so, up to 16 waves, where a lane takes up to four.
-  const int64_t chunks = uk::ceil_div(a.padded_cols, kChunk);
-  const int most = a.tiled_rows >= 1024 ? 2 : 1;
+  // Waves a row: as many as leave a lane with one chunk, up to eight; then more chunks a lane,
+  // and sixteen waves where those are too many. us with four / eight / sixteen waves: norm 2048 x
+  // 4096 14.5 / 16.2 / 23.4, 2048 x 8192 30.2 / 28.6 / 31.8; gate 2048 x 14336 37.8 / 33.6 / 38.2, 2048
+  // x 28672 - / 64.7 / 71.1 (of workgroups of sixteen waves a unit holds one, of eight three). Rows
+  // that leave units idle take sixteen before they take a second chunk: gate 16 x 14336 - / 7.3 /
+  // 6.4.
+  const int64_t chunks = uk::ceil_div(a.padded_cols, kChunk), most = p->norm ? 2 : 4;
+  const int up_to = a.tiled_rows <= 256 ? 4 : 3;
   int log_waves = 0;
-  while (log_waves < 4 && ((int64_t)most << (log_waves + 6)) < chunks) ++log_waves;
+  while (log_waves < up_to && ((int64_t)64 << log_waves) < chunks) ++log_waves;
+  if (most * (64 << log_waves) < chunks) log_waves = 4;
   const int64_t each = uk::ceil_div(chunks, (int64_t)64 << log_waves);
-  const bool in_registers = each <= 4;
+  const bool in_registers = each <= most;
   a.log_waves = log_waves;
   const int row_threads = 64 << log_waves;
   const int threads = row_threads < 256 && a.tiled_rows > 1 ? 256 : row_threads;
@@ -445,7 +474,7 @@ extern "C" int iree_uk_amd_hip_launch_row_op(const iree_uk_amd_row_op_t* p, void
       uk::launch(0, row_op_long_kernel<N, IN, F>, dim3((uint32_t)a.tiled_rows), dim3(kThreads), 0, stream, a);
       return;
     }
-    auto kernel = each <= 1 ? row_op_kernel<N, IN, F, 1> : each <= 2 ? row_op_kernel<N, IN, F, 2> : row_op_kernel<N, IN, F, 4>;
+    auto kernel = each <= 1 ? row_op_kernel<N, IN, F, 1> : each <= 2 ? row_op_kernel<N, IN, F, 2> : row_op_kernel<N, IN, F, N ? 2 : 4>;
     uk::launch(0, kernel, dim3((uint32_t)uk::ceil_div(a.tiled_rows, a.rows_a_block)), dim3((uint32_t)threads), 0, stream, a);
   };
   auto by_form = [&](auto norm, auto in_type) {

@@ -6,6 +6,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "iree_uk_amd.h"
 
 namespace uk {
@@ -17,6 +19,23 @@ namespace uk {
 // result to about three, and to |t| units where t is large and negative.
 __device__ __forceinline__ float times_sigmoid(float x, float t) {
   return x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504f * t));
+}
+
+// The same to about one unit: what an 8-bit form is made of, in which every unit more moves
+// some elements across the middle between two steps (f8 2048 x 28672 with the other one: twice
+// as far from the 64-bit result as with correctly rounded steps; gate_pack 64.7 us, so 67.9). The
+// exponent's rounding is carried along as a second term, and a Newton step takes the
+// reciprocal's away.
+__device__ __forceinline__ float times_sigmoid_close(float x, float t) {
+  constexpr float kLog2e = 1.44269502f, kLog2eRest = 1.92596299e-8f, kLn2 = 0.693147181f;
+  constexpr float kMost = 87.3365448f;   // 126 ln 2: the smallest sigmoid that is a normal f32
+  t = __builtin_amdgcn_fmed3f(t, -kMost, kMost);
+  const float hi = -kLog2e * t;
+  const float lo = __builtin_fmaf(-kLog2eRest, t, __builtin_fmaf(-kLog2e, t, -hi));
+  const float e = __builtin_amdgcn_exp2f(hi);
+  const float d = 1.0f + __builtin_fmaf(e, lo * kLn2, e);
+  const float r = __builtin_amdgcn_rcpf(d);
+  return x * __builtin_fmaf(__builtin_fmaf(-d, r, 1.0f), r, r);
 }
 
 // x Phi(x) with Phi(x) = erfc(-x / sqrt 2) / 2, by the approximation of Hastings that
@@ -38,7 +57,9 @@ __device__ __forceinline__ float gelu(float x) {
 
 // `act` is an IREE_UK_AMD_FLAG_ACTIVATION_* value, the same in all lanes. The comparison of
 // RELU lets a NaN through.
+template <bool CLOSE = false>
 __device__ __forceinline__ float activate(float x, uint32_t act) {
+  auto times_sigmoid = [](float v, float t) { return CLOSE ? times_sigmoid_close(v, t) : uk::times_sigmoid(v, t); };
   switch (act) {
     case IREE_UK_AMD_FLAG_ACTIVATION_RELU: return x < 0.0f ? 0.0f : x;
     case IREE_UK_AMD_FLAG_ACTIVATION_GELU: return gelu(x);
@@ -51,18 +72,18 @@ __device__ __forceinline__ float activate(float x, uint32_t act) {
 }
 
 // The activation of N elements, by one test of the activation for all of them.
-template <int N>
+template <bool CLOSE = false, int N>
 __device__ __forceinline__ void activate_all(float (&z)[N], uint32_t act) {
-  auto each = [&](auto f) __attribute__((always_inline)) {
+  auto each = [&](auto act_c) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) z[i] = f(z[i]);
+    for (int i = 0; i < N; ++i) z[i] = activate<CLOSE>(z[i], decltype(act_c)::value);
   };
   if (act == IREE_UK_AMD_FLAG_ACTIVATION_NONE) return;
-  if (act == IREE_UK_AMD_FLAG_ACTIVATION_SILU) each([](float x) { return activate(x, IREE_UK_AMD_FLAG_ACTIVATION_SILU); });
+  if (act == IREE_UK_AMD_FLAG_ACTIVATION_SILU) each(std::integral_constant<uint32_t, IREE_UK_AMD_FLAG_ACTIVATION_SILU>{});
   else if (act == IREE_UK_AMD_FLAG_ACTIVATION_GELU_TANH)
-    each([](float x) { return activate(x, IREE_UK_AMD_FLAG_ACTIVATION_GELU_TANH); });
-  else if (act == IREE_UK_AMD_FLAG_ACTIVATION_GELU) each([](float x) { return activate(x, IREE_UK_AMD_FLAG_ACTIVATION_GELU); });
-  else each([](float x) { return activate(x, IREE_UK_AMD_FLAG_ACTIVATION_RELU); });
+    each(std::integral_constant<uint32_t, IREE_UK_AMD_FLAG_ACTIVATION_GELU_TANH>{});
+  else if (act == IREE_UK_AMD_FLAG_ACTIVATION_GELU) each(std::integral_constant<uint32_t, IREE_UK_AMD_FLAG_ACTIVATION_GELU>{});
+  else each(std::integral_constant<uint32_t, IREE_UK_AMD_FLAG_ACTIVATION_RELU>{});
 }
 
 // f32 to and from the 16-bit floats, rounded to nearest even, subnormals kept.
