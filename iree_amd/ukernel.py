@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libiree_uk_amd.so")
@@ -107,6 +108,12 @@ class Mmt4dParams(ctypes.Structure):
                 ("K0", _i32), ("flags", _u32), ("cpu_data", _vp)]
 
 
+# iree_uk_amd_rmsnorm_pack_params_t, iree_uk_amd_gate_pack_params_t and
+# iree_uk_amd_mmt4d_epilogue_unpack_params_t (include/iree_uk_amd.h), field by field.
+_RMSNORM_PACK_PARAMS = struct.Struct("@PqqPqqPqqPfPqqPqqqqqqIP").pack
+_GATE_PACK_PARAMS = struct.Struct("@PqqPqqPqqPqqqqqqIP").pack
+_EPILOGUE_UNPACK_PARAMS = struct.Struct("@PqqPqqPqqPqqqqPPPqqqiiiIIP").pack
+
 ASSERT_HANDLER = ctypes.CFUNCTYPE(None, ctypes.c_char_p, ctypes.c_int,
                                   ctypes.c_char_p, ctypes.c_char_p)
 
@@ -175,15 +182,14 @@ class UKernelLibrary:
             [_vp, _i64, _i64] * 4 + [_i64, _i64, _vp, _vp, _i64, _i64, _i64,
                                      _i32, _i32, _i32, _u32, _vp])
         L.iree_uk_amd_mmt4d_dequant_unpack.restype = None
-        L.iree_uk_amd_mmt4d_epilogue_unpack.argtypes = (
-            [_vp, _i64, _i64] * 4 + [_i64, _i64, _vp, _vp, _vp, _i64, _i64, _i64,
-                                     _i32, _i32, _i32, _u32, _u32, _vp])
-        L.iree_uk_amd_mmt4d_epilogue_unpack.restype = None
-        L.iree_uk_amd_rmsnorm_pack.argtypes = (
-            [_vp, _i64, _i64] * 3 + [_vp, ctypes.c_float] + [_vp, _i64, _i64, _vp] + [_i64] * 6 + [_u32, _vp])
-        L.iree_uk_amd_rmsnorm_pack.restype = None
-        L.iree_uk_amd_gate_pack.argtypes = [_vp, _i64, _i64] * 3 + [_vp] + [_i64] * 6 + [_u32, _vp]
-        L.iree_uk_amd_gate_pack.restype = None
+        # Calls of short kernels: through the params structs, packed at once (24
+        # arguments converted one by one take 2.6 us of a call's 3.1, so 0.9).
+        self._mmt4d_epilogue_unpack_p = L.iree_uk_amd_mmt4d_epilogue_unpack_p
+        self._rmsnorm_pack_p = L.iree_uk_amd_rmsnorm_pack_p
+        self._gate_pack_p = L.iree_uk_amd_gate_pack_p
+        for f in (self._mmt4d_epilogue_unpack_p, self._rmsnorm_pack_p, self._gate_pack_p):
+            f.argtypes = [ctypes.c_char_p]
+            f.restype = None
         L.iree_uk_conv_nchwc.argtypes = ([_vp, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _i64,
                                           _vp, _i64, _i64, _i64, _i64] + [_i64] * 7 +
                                          [_i32] * 4 + [_u32, _vp])
@@ -329,10 +335,11 @@ class UKernelLibrary:
         """mmt4d into a row-major f32, f16 or bf16 matrix: residual +
         activation(product * row_scale * col_scale + bias). `epilogue_flags` is
         OUT_TYPE_* | ACTIVATION_*; residual, scales and bias may be None."""
-        self.lib.iree_uk_amd_mmt4d_epilogue_unpack(
-            lhs, lhs_offset, lhs_stride0, rhs, rhs_offset, rhs_stride0, residual, residual_offset,
-            residual_stride0, out, out_offset, out_stride0, out_size0, out_size1, row_scale,
-            col_scale, bias, M, N, K, M0, N0, K0, flags, epilogue_flags, cpu_data)
+        self._mmt4d_epilogue_unpack_p(_EPILOGUE_UNPACK_PARAMS(
+            lhs or 0, lhs_offset, lhs_stride0, rhs or 0, rhs_offset, rhs_stride0, residual or 0,
+            residual_offset, residual_stride0, out or 0, out_offset, out_stride0, out_size0, out_size1,
+            row_scale or 0, col_scale or 0, bias or 0, M, N, K, M0, N0, K0, flags, epilogue_flags,
+            cpu_data or 0))
         self._check()
 
     def rmsnorm_pack(self, inp, in_offset, in_stride0, residual, residual_offset, residual_stride0,
@@ -342,10 +349,11 @@ class UKernelLibrary:
         """Root-mean-square norm of in + residual, row by row, into the tiles of
         an mmt4d left-hand side, with a scale per row for the 8-bit types.
         `flags` is IN_TYPE_* | OUT_TYPE_*; residual, sum and weight may be None."""
-        self.lib.iree_uk_amd_rmsnorm_pack(
-            inp, in_offset, in_stride0, residual, residual_offset, residual_stride0, sum, sum_offset,
-            sum_stride0, weight, epsilon, out, out_offset, out_stride0, row_scale, in_size0, in_size1,
-            out_size0, out_size1, out_size2, out_size3, flags, cpu_data)
+        self._rmsnorm_pack_p(_RMSNORM_PACK_PARAMS(
+            inp or 0, in_offset, in_stride0, residual or 0, residual_offset, residual_stride0, sum or 0,
+            sum_offset, sum_stride0, weight or 0, epsilon, out or 0, out_offset, out_stride0,
+            row_scale or 0, in_size0, in_size1, out_size0, out_size1, out_size2, out_size3, flags,
+            cpu_data or 0))
         self._check()
 
     def gate_pack(self, gate, gate_offset, gate_stride0, up, up_offset, up_stride0, out, out_offset,
@@ -354,9 +362,10 @@ class UKernelLibrary:
         """activation(gate) * up into the tiles of an mmt4d left-hand side, with
         a scale per row for the 8-bit types. `flags` is IN_TYPE_* | OUT_TYPE_* |
         ACTIVATION_*; up may be None."""
-        self.lib.iree_uk_amd_gate_pack(
-            gate, gate_offset, gate_stride0, up, up_offset, up_stride0, out, out_offset, out_stride0,
-            row_scale, in_size0, in_size1, out_size0, out_size1, out_size2, out_size3, flags, cpu_data)
+        self._gate_pack_p(_GATE_PACK_PARAMS(
+            gate or 0, gate_offset, gate_stride0, up or 0, up_offset, up_stride0, out or 0, out_offset,
+            out_stride0, row_scale or 0, in_size0, in_size1, out_size0, out_size1, out_size2, out_size3,
+            flags, cpu_data or 0))
         self._check()
 
     def conv_nchwc(self, inp, input_offset, input_stride_n, input_stride_ic_outer,
