@@ -796,8 +796,9 @@ enum {
  * asked for; only with a residual) and may be in_buffer or residual_buffer
  * itself, with that one's offset and stride. weight: in_size1 entries of the in
  * type, or NULL. row_scale: in_size0 entries, for the 8-bit types, else not
- * used. out_stride0 >= 0, tile sizes as for iree_uk_pack; rows of sum and
- * row_scale beyond in_size0 stay as they are. */
+ * used. out_stride0 >= 0, tile sizes as for iree_uk_pack; out has no bytes in
+ * common with the other operands; rows of sum and entries of row_scale beyond
+ * in_size0 stay as they are. */
 typedef struct iree_uk_amd_rmsnorm_pack_params_t {
   const void* in_buffer;
   iree_uk_index_t in_offset;
@@ -887,14 +888,24 @@ IREE_UK_AMD_EXPORT void iree_uk_amd_gate_pack_p(
  *
  * evaluated in f32 from left to right (the sum with the bias and the product
  * with col_scale with or without a rounding in between) and rounded to the out
- * type once, at the end. row_scale, col_scale, bias: out_size0, out_size1
- * and out_size1 f32 entries; any of them may be NULL and then reads as 1, 1 and 0. residual_buffer: a matrix of the out type with
- * a stride of its own, or NULL; it may be the output itself (same offset and
- * stride), else the two do not overlap. Operand arguments, tile sizes and
- * `flags` are those of iree_uk_mmt4d for a type with a 32-bit accumulator,
- * without ACCUMULATE; `epilogue_flags` is out type | activation. K == 0 is a
- * product of zeros. out_size0 <= M*M0 and out_size1 <= N*N0; elements between
- * and behind the rows stay as they are. */
+ * type once, at the end. row_scale has out_size0, col_scale and bias have
+ * out_size1 f32 entries; any of them may be NULL and then reads as 1, 1 and 0.
+ * residual_buffer: a matrix of the out type with a stride of its own, or NULL;
+ * it may be the output itself (same offset and stride), else the two have no
+ * elements in common. Operand arguments, tile sizes and `flags` are those of
+ * iree_uk_mmt4d for a type with a 32-bit accumulator, without ACCUMULATE;
+ * `epilogue_flags` is out type | activation; strides of the matrices are not
+ * negative. K == 0 is a product of zeros. out_size0 <= M*M0 and out_size1 <=
+ * N*N0; elements between and behind the rows stay as they are.
+ *
+ * One launch, and no memory beyond the operands but what iree_uk_mmt4d keeps for
+ * the same product, for s8 (tile rows of 8 bytes and more), f16, bf16 and f8 (16
+ * bytes and more, what iree_uk_query_tile_sizes_2d answers with) and s8 x s4.
+ * Other types and tile rows run as a product into f32 and an epilogue of its
+ * own, in place for an f32 matrix, else from a buffer that the library keeps per
+ * thread and stream (64 MB, or one row of tiles; workspace_bytes and
+ * release_workspaces count it). On a stream that is being captured there is no
+ * such buffer and they take the scalar kernel: graphs want 16-byte tile rows. */
 typedef struct iree_uk_amd_mmt4d_epilogue_unpack_params_t {
   const void* lhs_buffer;
   iree_uk_index_t lhs_offset;

@@ -67,7 +67,13 @@ __device__ __forceinline__ void eight_bit_scale(float top, float r, float& scale
 //
 // `a.waves` waves a row (a power of two), a lane holding C chunks of 16 columns: a row is
 // read once, its reductions go over the lanes and, through LDS, over the waves, and what is
-// stored comes out of registers. Bound by memory.
+// stored comes out of registers.
+//
+// Bound by memory, with every byte moved once (measured: norm 2048 x 8192 bf16 into f8 reads
+// 67 MB and writes 49, gate 2048 x 28672 235 and 58): 28.6 us (4.1 TB/s) and 67.9 us (4.3 TB/s),
+// where a copy of 1 GiB moves 4.8 TB/s. The vector ALU is busy for 40 of those 67.9 us (25
+// instructions an element, the exponential and the reciprocal of SILU among them). Small
+// calls are the launch and one round trip: norm 1 x 4096 4.6 us, pack of as many bytes 4.0.
 constexpr int kChunk = 16;
 constexpr int kMaxThreads = 1024;
 
@@ -327,7 +333,8 @@ __global__ __launch_bounds__(kMaxThreads) void row_op_kernel(RowArgs a) {
 
 // ---- rows longer than what a workgroup's registers hold ---------------------------
 //
-// One workgroup a row, which it reads twice: for the two sums, and for the output.
+// One workgroup a row, which it reads twice: for the two sums, and for the output. (Columns are
+// counted without a sign: up to 2^31 - 1 of them, and a step more.)
 template <bool NORM, typename IN, Form FORM>
 __global__ __launch_bounds__(kThreads) void row_op_long_kernel(RowArgs a) {
   using T = typename IN::T;
@@ -335,16 +342,16 @@ __global__ __launch_bounds__(kThreads) void row_op_long_kernel(RowArgs a) {
   const uint32_t pm = a.by_m0.div(row), m0 = row - pm * (uint32_t)a.M0;
   constexpr int OB = FORM == Form::kSame ? (int)sizeof(T) : 1;
   char* out = a.out + (int64_t)pm * a.out_stride + (int64_t)m0 * a.K0 * OB;
-  auto at = [&](int c) {
-    const int64_t kt = a.by_k0.div((uint32_t)c);
+  auto at = [&](uint32_t c) {
+    const int64_t kt = a.by_k0.div(c);
     return out + (kt * a.M0 * a.K0 + (c - kt * a.K0)) * OB;
   };
-  auto put_zero = [&](int c) {
+  auto put_zero = [&](uint32_t c) {
     if constexpr (FORM == Form::kSame) *reinterpret_cast<T*>(at(c)) = IN::from_f32(0.0f);
     else *at(c) = 0;
   };
   if ((int)row >= a.rows) {
-    for (int c = threadIdx.x; c < a.padded_cols; c += kThreads) put_zero(c);
+    for (uint32_t c = threadIdx.x; c < (uint32_t)a.padded_cols; c += kThreads) put_zero(c);
     return;
   }
   const T* in = reinterpret_cast<const T*>(a.in + (int64_t)row * a.in_stride);
@@ -352,14 +359,14 @@ __global__ __launch_bounds__(kThreads) void row_op_long_kernel(RowArgs a) {
   T* sum = reinterpret_cast<T*>(a.sum + (int64_t)row * a.sum_stride);
   const T* weight = reinterpret_cast<const T*>(a.weight);
   // h of column c (norm), then u.
-  auto h_of = [&](int c) {
+  auto h_of = [&](uint32_t c) {
     float v = IN::to_f32(in[c]);
     if constexpr (NORM) {
       if (a.second) v += IN::to_f32(second[c]);
     }
     return v;
   };
-  auto u_of = [&](int c, float h) {
+  auto u_of = [&](uint32_t c, float h) {
     if constexpr (NORM) return a.weight ? h * IN::to_f32(weight[c]) : h;
     float v = uk::activate<true>(h, a.act);
     return a.second ? v * IN::to_f32(second[c]) : v;
@@ -368,7 +375,7 @@ __global__ __launch_bounds__(kThreads) void row_op_long_kernel(RowArgs a) {
   __shared__ uint32_t part_largest[kThreads];
   float squares = 0.0f;
   uint32_t largest = 0;
-  for (int c = threadIdx.x; c < a.cols; c += kThreads) {
+  for (uint32_t c = threadIdx.x; c < (uint32_t)a.cols; c += kThreads) {
     const float h = h_of(c);
     if constexpr (NORM) squares += h * h;
     if constexpr (FORM != Form::kSame) largest = larger(largest, u_of(c, h));
@@ -391,8 +398,8 @@ __global__ __launch_bounds__(kThreads) void row_op_long_kernel(RowArgs a) {
     eight_bit_scale<FORM>(__uint_as_float(part_largest[0]), r, scale, inverse);
     if (threadIdx.x == 0) a.row_scale[row] = scale;
   }
-  for (int c = threadIdx.x; c < a.padded_cols; c += kThreads) {
-    if (c >= a.cols) { put_zero(c); continue; }
+  for (uint32_t c = threadIdx.x; c < (uint32_t)a.padded_cols; c += kThreads) {
+    if (c >= (uint32_t)a.cols) { put_zero(c); continue; }
     const float h = h_of(c), u = u_of(c, h);
     // (Where sum is one of the inputs, this thread alone has read what it now overwrites.)
     if constexpr (NORM) {

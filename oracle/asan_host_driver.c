@@ -122,6 +122,54 @@ static void mmt4d_pitch_case(uint32_t type, int lb, int rb, int ob, int lhs_mode
   free(lhs); free(rhs); free(out_a); free(out_b);
 }
 
+/* Row-wise steps and the fused epilogue on host memory: buffers that hold exactly what the
+ * calls may touch, so that staging one byte more is an error. The stub kernel writes 7 to
+ * every byte of the tiles and the last byte of a row's inputs to its scale. */
+static void row_op_case(int es, uint32_t in_type, uint32_t out_type, int rows, int cols, int M0, int K0,
+                        int slack, int in_place) {
+  const int os = out_type == IREE_UK_AMD_FLAG_OUT_TYPE_S8 ? 1 : es;
+  const int64_t M1 = (rows + M0 - 1) / M0, K1 = (cols + K0 - 1) / K0, stride = cols + slack,
+                tiles = K1 * M0 * K0, ostride = tiles + slack, off = slack;
+  const size_t bytes = (size_t)(off + (rows ? (rows - 1) * stride + cols : 0)) * es;
+  uint8_t* in = random_bytes(bytes, 0);
+  uint8_t* second = random_bytes(bytes, 0);
+  uint8_t* sum = in_place ? in : random_bytes(bytes, 0);
+  uint8_t* weight = random_bytes((size_t)cols * es, 0);
+  const size_t out_bytes = (size_t)(off + (M1 ? (M1 - 1) * ostride + tiles : 0)) * os;
+  uint8_t* out = random_bytes(out_bytes, 0);
+  uint8_t* before = clone(out, out_bytes);
+  float* scale = (float*)random_bytes((size_t)rows * 4, 0);
+  for (int gate = 0; gate < 2; ++gate) {
+    if (gate) {
+      iree_uk_amd_gate_pack(in, off, stride, second, off, stride, out, off, ostride, os == 1 ? scale : 0, rows, cols, M1,
+                            K1, M0, K0, in_type | out_type | IREE_UK_AMD_FLAG_ACTIVATION_SILU, 0);
+    } else {
+      iree_uk_amd_rmsnorm_pack(in, off, stride, second, off, stride, sum, off, stride, weight, 1e-5f, out, off, ostride,
+                               os == 1 ? scale : 0, rows, cols, M1, K1, M0, K0, in_type | out_type, 0);
+    }
+    CHECK(iree_uk_amd_last_status() == 0);
+    for (int64_t i = 0; i < (int64_t)out_bytes / os; ++i) {
+      const int64_t at = i - off;
+      const int inside = at >= 0 && at % ostride < tiles;
+      for (int b = 0; b < os; ++b) CHECK(out[i * os + b] == (inside ? 7 : before[i * os + b]));
+    }
+  }
+  /* The fused epilogue: everything is staged, then the stub has no kernel for it. */
+  if (es == 4 && rows && cols) {
+    uint8_t* lhs = random_bytes((size_t)rows * 16, 0);
+    uint8_t* rhs = random_bytes((size_t)cols * 16, 0);
+    float* bias = (float*)random_bytes((size_t)cols * 4, 0);
+    iree_uk_amd_mmt4d_epilogue_unpack(lhs, 0, 16, rhs, 0, 16, second, off, stride, in, off, stride, rows, cols, scale, bias,
+                                      bias, rows, cols, 1, 1, 1, 16,
+                                      IREE_UK_FLAG_MMT4D_TYPE_S8S8S32 | IREE_UK_FLAG_MMT4D_ALLOW_GENERIC_FALLBACK_TILE_FUNCTION,
+                                      IREE_UK_AMD_FLAG_OUT_TYPE_F32 | IREE_UK_AMD_FLAG_ACTIVATION_GELU, 0);
+    CHECK(iree_uk_amd_last_status() != 0);
+    free(lhs); free(rhs); free(bias);
+  }
+  if (!in_place) free(sum);
+  free(in); free(second); free(weight); free(out); free(before); free(scale);
+}
+
 static void pack_unpack_case(uint32_t type, int es, int rows, int cols, int t0, int t1,
                              uint32_t transpose, int slack) {
   const int inner = (transpose & IREE_UK_FLAG_PACK_TRANSPOSE_INNER) != 0;
@@ -219,6 +267,14 @@ int main(void) {
       mmt4d_case(IREE_UK_FLAG_MMT4D_TYPE_S16S16S32, 16, 16, 32, 2, 2, 3, 4, 4, 2, acc, slack);
       mmt4d_case(IREE_UK_FLAG_MMT4D_TYPE_S8S4S32, 8, 4, 32, 2, 3, 2, 4, 8, 4, acc, slack);
       mmt4d_case(IREE_UK_FLAG_MMT4D_TYPE_S8S8S32, 8, 8, 32, 2, 2, 0, 4, 4, 2, acc, slack);
+    }
+  }
+  for (int slack = 0; slack <= 3; slack += 3) {
+    for (int in_place = 0; in_place < 2; ++in_place) {
+      row_op_case(2, IREE_UK_AMD_FLAG_IN_TYPE_BF16, IREE_UK_AMD_FLAG_OUT_TYPE_S8, 5, 37, 4, 16, slack, in_place);
+      row_op_case(2, IREE_UK_AMD_FLAG_IN_TYPE_F16, IREE_UK_AMD_FLAG_OUT_TYPE_F16, 1, 1, 1, 3, slack, in_place);
+      row_op_case(4, IREE_UK_AMD_FLAG_IN_TYPE_F32, IREE_UK_AMD_FLAG_OUT_TYPE_S8, 17, 8, 16, 8, slack, in_place);
+      row_op_case(4, IREE_UK_AMD_FLAG_IN_TYPE_F32, IREE_UK_AMD_FLAG_OUT_TYPE_F32, 2, 9, 1, 4, slack, in_place);
     }
   }
   CHECK(violations == 0);

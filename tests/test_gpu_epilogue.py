@@ -134,6 +134,51 @@ def test_epilogue_of_layer_sizes(gpu, type_, M0, N0, K0, rows, cols, k):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("type_,M0,N0,K0", [(S8, 16, 16, 16), (F8, 16, 16, 32), (BF16, 1, 16, 8), (F16, 24, 12, 8)])
+def test_epilogue_with_rows_at_any_address(gpu, type_, M0, N0, K0):
+    """Rows of whole groups of columns at odd pitches and offsets, in every kernel: what loads and stores
+    16 bytes at once does so at any address of an element. Panels that do not divide a block (M0 = 24)."""
+    lib, _ = gpu
+    for i, (rows, cols, k) in enumerate([(1, 512, 1024), (40, 264, 100), (70, 1024, 512), (300, 512, 640), (520, 776, 320),
+                                         (1024, 2048, 256), (2050, 2056, 200), (4096, 4096, 96)]):
+        for j, (out, pitch, offset) in enumerate([("bf16", 1, 1), ("f32", 3, 1), ("f16", 8, 3)]):
+            run(lib, type_, rows, cols, k, M0, N0, K0, out, list(ACTS)[(i + j) % 5], pitch=pitch, offset=offset,
+                residual=("own", "in place", None)[(i + j) % 3], scales=i % 2 == 0, seed=i)
+
+
+@pytest.mark.gpu
+def test_epilogue_of_4_bit_weights(gpu):
+    """s8 x s4, both in the kernel for few rows and on expanded weights, and the widened s16 x s8: types with a
+    right-hand side of another width than the left-hand one's."""
+    lib, _ = gpu
+    rng = np.random.default_rng(3)
+    for rows, cols, k, K0 in [(1, 512, 1024, 16), (40, 300, 512, 32), (70, 512, 448, 32), (600, 256, 512, 16), (5, 40, 96, 8)]:
+        N1, K1 = -(-cols // 16), -(-k // K0)
+        a = rng.integers(-8, 9, (rows, k))
+        b = np.zeros((N1 * 16, K1 * K0), np.int64)
+        b[:cols, :k] = rng.integers(-8, 8, (cols, k))
+        t = b.reshape(N1, 16, K1, K0).transpose(0, 2, 1, 3).reshape(-1, 2) & 15
+        rhs = torch.from_numpy((t[:, 0] | t[:, 1] << 4).astype(np.uint8)).cuda()
+        full = np.zeros((rows, K1 * K0), np.int8)
+        full[:, :k] = a
+        lhs = torch.from_numpy(full).cuda()
+        cs = torch.rand(cols, device="cuda") * 0.01
+        res = torch.randn(rows, cols, device="cuda").to(torch.bfloat16)
+        out = torch.zeros(rows, cols, device="cuda", dtype=torch.bfloat16)
+        lib.mmt4d_epilogue_unpack(lhs.data_ptr(), 0, K1 * K0, rhs.data_ptr(), 0, K1 * 16 * K0, res.data_ptr(), 0, cols,
+                                  out.data_ptr(), 0, cols, rows, cols, None, cs.data_ptr(), None, rows, N1, K1, 1, 16, K0,
+                                  uk.MMT4D_TYPE_S8S4S32 | uk.MMT4D_ALLOW_GENERIC_FALLBACK_TILE_FUNCTION,
+                                  uk.OUT_TYPE_BF16 | uk.ACTIVATION_RELU)
+        lib.synchronize()
+        z = (a @ b[:cols, :k].T) * cs.cpu().double().numpy()
+        want = np.maximum(z, 0) + res.cpu().double().numpy()
+        half, tiny = HALF["bf16"]
+        off = np.abs(out.cpu().double().numpy() - want) - (np.abs(want) * half + (4 * U32 * np.abs(z) + 2 * U32 * np.abs(want)) * 2
+                                                           + tiny)
+        assert off.max() <= 0, (rows, cols, k, lib.last_kernel_name(), off.max())
+
+
+@pytest.mark.gpu
 def test_epilogue_of_a_product_over_no_k(gpu):
     """K == 0: what the epilogue makes of zeros."""
     lib, _ = gpu
