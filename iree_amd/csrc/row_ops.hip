@@ -65,8 +65,9 @@ __device__ __forceinline__ void eight_bit_scale(float top, float r, float& scale
 
 // ---- rows in registers ---------------------------------------------------------
 //
-// `a.waves` waves a row (a power of two), a lane holding C chunks of 16 columns: a row is
-// read once, its reductions go over the lanes and, through LDS, over the waves, and what is
+// 2^a.log_waves waves a row, a lane holding C chunks of 8 columns, one 16-byte load of a 16-bit
+// type (chunks of two loads each, whose lanes lie 32 bytes apart: norm 2048 x 8192 bf16 28.8 us, so
+// 26.2, 2000 x 5001 gated 20.0 / 17.8): a row is read once, its reductions go over the lanes and, through LDS, over the waves, and what is
 // stored comes out of registers.
 //
 // Bound by memory, with every byte moved once (measured: norm 2048 x 8192 bf16 into f8 reads
@@ -74,7 +75,7 @@ __device__ __forceinline__ void eight_bit_scale(float top, float r, float& scale
 // where a copy of 1 GiB moves 4.8 TB/s. The vector ALU is busy for 40 of those 67.9 us (25
 // instructions an element, the exponential and the reciprocal of SILU among them). Small
 // calls are the launch and one round trip: norm 1 x 4096 4.6 us, pack of as many bytes 4.0.
-constexpr int kChunk = 16;
+constexpr int kChunk = 8;
 constexpr int kMaxThreads = 1024;
 
 template <typename T, int N>
@@ -83,13 +84,13 @@ struct Any {
   typedef V At __attribute__((aligned(sizeof(T))));   // at any address of its elements
 };
 
-// Columns c .. c + 15 of a row as they lie in memory. Loading and using them are two steps,
+// Columns c .. c + 7 of a row as they lie in memory. Loading and using them are two steps,
 // and no lane branches in the first: what a kernel loads is then in flight together, one
 // round trip to memory where `load, convert` for each of residual and weight made three.
 template <typename IN>
 struct Chunk {
   using T = typename IN::T;
-  static constexpr int PIECES = (int)sizeof(T), N = kChunk / PIECES;   // of 16 bytes; columns of one
+  static constexpr int PIECES = (int)sizeof(T) / 2, N = kChunk / PIECES;   // of 16 bytes; columns of one
   uint32_t w[PIECES][4];
 
   // `row_bytes` > 0: of the row. A piece beyond its end is loaded from its last 16 bytes.
@@ -121,8 +122,8 @@ struct Chunk {
   }
 };
 
-// 16 elements of OB bytes, in words, to the tiles of a row: `at(column)` is where a column
-// goes. Runs of `piece` columns lie next to each other (16, 8, 4, or else single ones).
+// The elements of a chunk, of OB bytes, in words, to the tiles of a row: `at(column)` is where a column
+// goes. Runs of `piece` columns lie next to each other (8, 4, or else single ones).
 template <int OB, typename At>
 __device__ __forceinline__ void store_chunk(const uint32_t (&w)[kChunk * OB / 4], int c, int padded_cols, int piece, At at) {
   typedef uint32_t v4u __attribute__((ext_vector_type(4)));
@@ -145,8 +146,7 @@ __device__ __forceinline__ void store_chunk(const uint32_t (&w)[kChunk * OB / 4]
           *reinterpret_cast<v4u_any*>(p + 4 * i) = v4u{w[first + i], w[first + i + 1], w[first + i + 2], w[first + i + 3]};
     }
   };
-  if (piece == 16) store_run(std::integral_constant<int, 16>{});
-  else if (piece == 8) store_run(std::integral_constant<int, 8>{});
+  if (piece == 8) store_run(std::integral_constant<int, 8>{});
   else if (piece == 4) store_run(std::integral_constant<int, 4>{});
   else {
 #pragma unroll
@@ -187,8 +187,8 @@ __global__ __launch_bounds__(kMaxThreads) void row_op_kernel(RowArgs a) {
   uint32_t largest = 0;
   const uint32_t row_bytes = (uint32_t)a.cols * (uint32_t)sizeof(T);
   if (exists && a.cols > 0) {   // (the same in all lanes of a wave)
-    // (Four chunks, of gates only, one after the other: their registers.)
-    constexpr int P = C <= 2 ? C : 1;
+    // (Up to four chunks together: the registers of more.)
+    constexpr int P = C <= 4 ? C : 4;
     Chunk<IN> x[P], y[P], z[NORM ? P : 1];
 #pragma unroll
     for (int i = 0; i < C; ++i) {
@@ -455,16 +455,17 @@ extern "C" int iree_uk_amd_hip_launch_row_op(const iree_uk_amd_row_op_t* p, void
   }
   hipStream_t stream = (hipStream_t)stream_v;
   *kernel_name = p->norm ? "rmsnorm_pack" : "gate_pack";
-  // Waves a row: as many as leave a lane with one chunk, up to eight; then more chunks a lane,
+  // Waves a row: as many as leave a lane with two chunks, up to eight; then more chunks a lane,
   // and sixteen waves where those are too many. us with four / eight / sixteen waves: norm 2048 x
-  // 4096 14.5 / 16.2 / 23.4, 2048 x 8192 30.2 / 28.6 / 31.8; gate 2048 x 14336 37.8 / 33.6 / 38.2, 2048
-  // x 28672 - / 64.7 / 71.1 (of workgroups of sixteen waves a unit holds one, of eight three). Rows
-  // that leave units idle take sixteen before they take a second chunk: gate 16 x 14336 - / 7.3 /
-  // 6.4.
-  const int64_t chunks = uk::ceil_div(a.padded_cols, kChunk), most = p->norm ? 2 : 4;
-  const int up_to = a.tiled_rows <= 256 ? 4 : 3;
+  // 4096 bf16 13.7 / 13.6 / -, 2048 x 8192 32.3 / 29.2 / 27.6, gate 2048 x 14336 37.5 / 35.0 / 34.1, 2048 x
+  // 28672 - / 68.4 / 76.3. f32, whose chunks are two loads: as many as leave it with one, up to
+  // sixteen (norm 2048 x 4096 31.4 / 26.7 / 27.7, gate 2048 x 8192 59.0 / 60.1 / 49.8). Rows that leave
+  // units idle take sixteen before they take a third chunk: gate 16 x 14336 8.6 / 7.3 / 7.0.
+  const int64_t chunks = uk::ceil_div(a.padded_cols, kChunk), most = p->norm ? 4 : 8;
+  const int64_t wanted = es == 4 ? 1 : 2;
+  const int up_to = es == 4 || a.tiled_rows <= 256 ? 4 : 3;
   int log_waves = 0;
-  while (log_waves < up_to && ((int64_t)64 << log_waves) < chunks) ++log_waves;
+  while (log_waves < up_to && (wanted * 64 << log_waves) < chunks) ++log_waves;
   if (most * (64 << log_waves) < chunks) log_waves = 4;
   const int64_t each = uk::ceil_div(chunks, (int64_t)64 << log_waves);
   const bool in_registers = each <= most;
@@ -472,7 +473,7 @@ extern "C" int iree_uk_amd_hip_launch_row_op(const iree_uk_amd_row_op_t* p, void
   const int row_threads = 64 << log_waves;
   const int threads = row_threads < 256 && a.tiled_rows > 1 ? 256 : row_threads;
   a.rows_a_block = threads / row_threads;
-  a.piece = (int32_t)uk::pow2_divisor(a.K0, 16);
+  a.piece = (int32_t)uk::pow2_divisor(a.K0, 8);
   auto go = [&](auto norm, auto in_type, auto form_c) {
     constexpr bool N = decltype(norm)::value;
     constexpr Form F = decltype(form_c)::value;
@@ -481,7 +482,7 @@ extern "C" int iree_uk_amd_hip_launch_row_op(const iree_uk_amd_row_op_t* p, void
       uk::launch(0, row_op_long_kernel<N, IN, F>, dim3((uint32_t)a.tiled_rows), dim3(kThreads), 0, stream, a);
       return;
     }
-    auto kernel = each <= 1 ? row_op_kernel<N, IN, F, 1> : each <= 2 ? row_op_kernel<N, IN, F, 2> : row_op_kernel<N, IN, F, N ? 2 : 4>;
+    auto kernel = each <= 1 ? row_op_kernel<N, IN, F, 1> : each <= 2 ? row_op_kernel<N, IN, F, 2> : each <= 4 ? row_op_kernel<N, IN, F, 4> : row_op_kernel<N, IN, F, N ? 4 : 8>;
     uk::launch(0, kernel, dim3((uint32_t)uk::ceil_div(a.tiled_rows, a.rows_a_block)), dim3((uint32_t)threads), 0, stream, a);
   };
   auto by_form = [&](auto norm, auto in_type) {
