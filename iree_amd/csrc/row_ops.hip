@@ -65,16 +65,18 @@ __device__ __forceinline__ void eight_bit_scale(float top, float r, float& scale
 
 // ---- rows in registers ---------------------------------------------------------
 //
-// 2^a.log_waves waves a row, a lane holding C chunks of 8 columns, one 16-byte load of a 16-bit
-// type (chunks of two loads each, whose lanes lie 32 bytes apart: norm 2048 x 8192 bf16 28.8 us, so
-// 26.2, 2000 x 5001 gated 20.0 / 17.8): a row is read once, its reductions go over the lanes and, through LDS, over the waves, and what is
-// stored comes out of registers.
+// 2^a.log_waves waves a row, a lane holding C chunks of 8 columns, one 16-byte load of a
+// 16-bit type, so that the loads of a wave cover neighbouring lines (chunks of two loads, whose
+// lanes lie 32 bytes apart: norm 2048 x 8192 bf16 28.8 us, this 26.2; gate 2000 x 5001 17.8 and
+// 16.0). A row is read once, its reductions go over the lanes and, through LDS, over the waves,
+// and what is stored comes out of registers.
 //
 // Bound by memory, with every byte moved once (measured: norm 2048 x 8192 bf16 into f8 reads
-// 67 MB and writes 49, gate 2048 x 28672 235 and 58): 28.6 us (4.1 TB/s) and 67.9 us (4.3 TB/s),
-// where a copy of 1 GiB moves 4.8 TB/s. The vector ALU is busy for 40 of those 67.9 us (25
-// instructions an element, the exponential and the reciprocal of SILU among them). Small
-// calls are the launch and one round trip: norm 1 x 4096 4.6 us, pack of as many bytes 4.0.
+// 67 MB and writes 49, gate 2048 x 28672 235 and 58): 26.2 us (4.5 TB/s) and 66.0 us (4.4 TB/s),
+// where a copy of 1 GiB by torch moves 4.8 TB/s, by the best of the kernels tried 5.8. The
+// vector ALU is busy for over half of the gate's time (the exponential and the reciprocal of
+// SILU). Small calls are the launch and one round trip: norm 1 x 4096 4.6 us, pack of as many
+// bytes 4.0.
 constexpr int kChunk = 8;
 constexpr int kMaxThreads = 1024;
 

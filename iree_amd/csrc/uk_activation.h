@@ -36,20 +36,24 @@ __device__ __forceinline__ float times_sigmoid_close(float x, float t) {
   return x * __builtin_amdgcn_rcpf(__builtin_fmaf(e, lo, 1.0f + e));
 }
 
-// x Phi(x) with Phi(x) = erfc(-x / sqrt 2) / 2, by the approximation of Hastings that
-// Abramowitz and Stegun give as 7.1.26 (erfc(z) = e^(-z^2) p(t), t = 1 / (1 + 0.3275911 z),
-// to 1.5e-7 for z >= 0): x - x erfc(z) / 2 for positive x, x erfc(z) / 2 for negative,
-// so nothing cancels in the negative tail.
+// x Phi(x) with Phi(x) = erfc(-x / sqrt 2) / 2. With s = |x| and tail = s erfc(s / sqrt 2) / 2
+// it is s - tail for positive x and -tail for negative, so nothing cancels in the negative tail.
+// erfc(s / sqrt 2) / 2 = e^(-s^2 / 2) p(t) with t = 1 / (1 + 0.4 s / sqrt 2), and p, without a
+// constant term, was fitted for the smallest largest error of the tail: 5.8e-9 for all s, and with
+// the roundings of f32 2.7e-7 |x| at most, 3e-8 of the root mean square for normal x.
+// (Of 10 million 8-bit roundings 3 are not those of exact values; with five terms, to 1.7e-7
+// at their best, 5. erfcf is closer yet, at branches between lanes: gate 2048 x 28672
+// 114 us where this takes 75.)
 __device__ __forceinline__ float gelu(float x) {
   // (From 64 on the tail is zero, an infinite x, whose tail would be infinity times zero, among them.)
-  const float ax = __builtin_fminf(__builtin_fabsf(x), 64.0f);
-  const float z = ax * 0.70710678f;
-  const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f, z, 1.0f));
-  float p = __builtin_fmaf(1.061405429f, t, -1.453152027f);
-  p = __builtin_fmaf(p, t, 1.421413741f);
-  p = __builtin_fmaf(p, t, -0.284496736f);
-  p = __builtin_fmaf(p, t, 0.254829592f);
-  const float tail = 0.5f * ax * (p * t * __builtin_amdgcn_exp2f(-1.44269504f * z * z));
+  const float s = __builtin_fminf(__builtin_fabsf(x), 64.0f);
+  const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.282842726f, s, 1.0f));
+  float p = __builtin_fmaf(-0.103000157f, t, 0.36618006f);
+  p = __builtin_fmaf(p, t, -0.204105198f);
+  p = __builtin_fmaf(p, t, 0.249023885f);
+  p = __builtin_fmaf(p, t, 0.0750114322f);
+  p = __builtin_fmaf(p, t, 0.116889864f);
+  const float tail = s * (p * t * __builtin_amdgcn_exp2f(-0.72134752f * s * s));
   return (x < 0.0f ? 0.0f : x) - tail;   // (a NaN is not below zero, and stays)
 }
 
