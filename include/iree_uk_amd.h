@@ -796,9 +796,11 @@ enum {
  * asked for; only with a residual) and may be in_buffer or residual_buffer
  * itself, with that one's offset and stride. weight: in_size1 entries of the in
  * type, or NULL. row_scale: in_size0 entries, for the 8-bit types, else not
- * used. out_stride0 >= 0, tile sizes as for iree_uk_pack; out has no bytes in
- * common with the other operands; rows of sum and entries of row_scale beyond
- * in_size0 stay as they are. */
+ * used. Rows of sum and of out do not overlap (strides of a row and more), tile
+ * sizes are as for iree_uk_pack; out has no bytes in common with the other
+ * operands; rows of sum and entries of row_scale beyond in_size0 stay as they
+ * are. An epsilon of 0 is for rows whose squares f32 holds: where their mean is
+ * zero, y is NaN or infinite. */
 typedef struct iree_uk_amd_rmsnorm_pack_params_t {
   const void* in_buffer;
   iree_uk_index_t in_offset;
@@ -894,8 +896,8 @@ IREE_UK_AMD_EXPORT void iree_uk_amd_gate_pack_p(
  * it may be the output itself (same offset and stride), else the two have no
  * elements in common. Operand arguments, tile sizes and `flags` are those of
  * iree_uk_mmt4d for a type with a 32-bit accumulator, without ACCUMULATE;
- * `epilogue_flags` is out type | activation; strides of the matrices are not
- * negative. K == 0 is a product of zeros. out_size0 <= M*M0 and out_size1 <=
+ * `epilogue_flags` is out type | activation; out_stride0 >= out_size1 (where
+ * there is more than one row), residual_stride0 >= 0. K == 0 is a product of zeros. out_size0 <= M*M0 and out_size1 <=
  * N*N0; elements between and behind the rows stay as they are.
  *
  * One launch, and no memory beyond the operands but what iree_uk_mmt4d keeps for

@@ -104,7 +104,7 @@ int launch_epilogue_apart(const iree_uk_mmt4d_params_t* p, const iree_uk_amd_row
   a.ep.bias = rm->bias;
   a.ep.residual_pitch = rm->residual_stride0 * a.ep.out_bytes;
   const int64_t row_bytes = rm->size1 * a.ep.out_bytes;
-  const bool in_place = a.ep.out_bytes == 4 && (a.ep.out_pitch >= row_bytes || rm->size0 == 1) &&
+  const bool in_place = a.ep.out_bytes == 4 &&
                         !(rm->residual && overlaps((const char*)p->out_buffer, (rm->size0 - 1) * a.ep.out_pitch + row_bytes,
                                                    (const char*)rm->residual,
                                                    (rm->size0 - 1) * a.ep.residual_pitch + row_bytes));

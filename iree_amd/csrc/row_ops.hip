@@ -480,12 +480,29 @@ extern "C" int iree_uk_amd_hip_launch_row_op(const iree_uk_amd_row_op_t* p, void
     constexpr bool N = decltype(norm)::value;
     constexpr Form F = decltype(form_c)::value;
     using IN = decltype(in_type);
-    if (!in_registers) {
-      uk::launch(0, row_op_long_kernel<N, IN, F>, dim3((uint32_t)a.tiled_rows), dim3(kThreads), 0, stream, a);
-      return;
+    auto kernel = each <= 1   ? row_op_kernel<N, IN, F, 1>
+                  : each <= 2 ? row_op_kernel<N, IN, F, 2>
+                  : each <= 4 ? row_op_kernel<N, IN, F, 4>
+                              : row_op_kernel<N, IN, F, N ? 4 : 8>;
+    // A grid has fewer than 2^32 threads: whole tiles of up to 2^21 rows a launch (a tile
+    // has 4096 bytes at most, so 4096 rows).
+    const int64_t most_panels = (1ll << 21) / p->M0;
+    for (int64_t m = 0; m < p->M1; m += most_panels) {
+      const int64_t first = m * p->M0, panels = p->M1 - m < most_panels ? p->M1 - m : most_panels;
+      RowArgs b = a;
+      b.in += first * a.in_stride;
+      if (a.second) b.second += first * a.second_stride;
+      if (a.sum) b.sum += first * a.sum_stride;
+      b.out += m * a.out_stride;
+      if (a.row_scale) b.row_scale += first;
+      b.rows = (int32_t)(p->rows > first ? p->rows - first : 0);
+      b.tiled_rows = (int32_t)(panels * p->M0);
+      if (b.rows > b.tiled_rows) b.rows = b.tiled_rows;
+      if (in_registers)
+        uk::launch(0, kernel, dim3((uint32_t)uk::ceil_div(b.tiled_rows, a.rows_a_block)), dim3((uint32_t)threads), 0, stream, b);
+      else
+        uk::launch(0, row_op_long_kernel<N, IN, F>, dim3((uint32_t)b.tiled_rows), dim3(kThreads), 0, stream, b);
     }
-    auto kernel = each <= 1 ? row_op_kernel<N, IN, F, 1> : each <= 2 ? row_op_kernel<N, IN, F, 2> : each <= 4 ? row_op_kernel<N, IN, F, 4> : row_op_kernel<N, IN, F, N ? 4 : 8>;
-    uk::launch(0, kernel, dim3((uint32_t)uk::ceil_div(a.tiled_rows, a.rows_a_block)), dim3((uint32_t)threads), 0, stream, a);
   };
   auto by_form = [&](auto norm, auto in_type) {
     if (form == Form::kS8) go(norm, in_type, std::integral_constant<Form, Form::kS8>{});

@@ -646,6 +646,10 @@ static int mmt4d_epilogue_validate(
   UK_REQUIRE(p->out_size0 >= 0 && p->out_size0 <= p->M * p->M0);
   UK_REQUIRE(p->out_size1 >= 0 && p->out_size1 <= p->N * p->N0);
   UK_REQUIRE(p->out_stride0 >= 0 && p->residual_stride0 >= 0);
+  UK_REQUIRE(p->out_size0 <= 1 || p->out_stride0 >= p->out_size1);
+  UK_REQUIRE(p->out_buffer || p->out_size0 == 0 || p->out_size1 == 0);
+  UK_REQUIRE((p->lhs_buffer && p->rhs_buffer) || p->out_size0 == 0 ||
+             p->out_size1 == 0 || p->K == 0 || p->K0 == 0);
   return 1;
 }
 
@@ -844,6 +848,11 @@ static int row_op_validate(const iree_uk_amd_row_op_t* p) {
   UK_REQUIRE(p->sum_stride0 >= 0 && p->out_stride0 >= 0);
   UK_REQUIRE(!is_8bit_type(out) || p->rows == 0 || p->row_scale != 0);
   UK_REQUIRE(!p->sum || p->second);
+  UK_REQUIRE(p->in || p->rows == 0 || p->cols == 0);
+  UK_REQUIRE(p->out || p->M1 * p->M0 == 0 || p->K1 * p->K0 == 0);
+  /* Rows that are written do not overlap. */
+  UK_REQUIRE(!p->sum || p->rows <= 1 || p->sum_stride0 >= p->cols);
+  UK_REQUIRE(p->M1 <= 1 || p->out_stride0 >= p->K1 * p->M0 * p->K0);
   UK_REQUIRE(!p->norm || p->epsilon >= 0.0f);
   return 1;
 }

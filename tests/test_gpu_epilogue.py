@@ -259,15 +259,16 @@ def test_epilogue_refusals(lib):
     """Needs no device."""
     lib.raise_on_violation(True)
 
-    def call(flags=S8, ep=uk.OUT_TYPE_BF16, rows=16, cols=16, M=1, stride=16, rstride=0):
-        lib.mmt4d_epilogue_unpack(None, 0, 0, None, 0, 0, None, 0, rstride, None, 0, stride, rows, cols, None, None, None, M, 1,
+    def call(flags=S8, ep=uk.OUT_TYPE_BF16, rows=16, cols=16, M=1, stride=16, rstride=0, lhs=64, rhs=64, dst=64):
+        lib.mmt4d_epilogue_unpack(lhs, 0, 0, rhs, 0, 0, None, 0, rstride, dst, 0, stride, rows, cols, None, None, None, M, 1,
                                   1, 16, 16, 16, flags, ep)
 
     for kw in [dict(flags=uk.MMT4D_TYPE_F16F16F16 | uk.MMT4D_SKIP_INTERMEDIATE_ROUNDINGS), dict(flags=0),
                dict(flags=S8 | uk.MMT4D_ACCUMULATE), dict(ep=0), dict(ep=uk.OUT_TYPE_S8), dict(ep=uk.OUT_TYPE_F8E4M3FN),
                dict(ep=uk.OUT_TYPE_F32 | 0x500), dict(ep=uk.OUT_TYPE_F32 | uk.IN_TYPE_F32), dict(ep=0x1010), dict(rows=17),
                dict(cols=17), dict(rows=-1), dict(stride=-16), dict(rstride=-1),
-               dict(flags=uk.MMT4D_TYPE_S16S8S32)]:
+               dict(flags=uk.MMT4D_TYPE_S16S8S32), dict(stride=15), dict(stride=0), dict(lhs=None), dict(rhs=None),
+               dict(dst=None)]:
         with pytest.raises(uk.ContractViolation):
             call(**kw)
     call(rows=0)

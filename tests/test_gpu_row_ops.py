@@ -377,16 +377,17 @@ def test_row_op_refusals(lib):
     lib.raise_on_violation(True)
 
     def norm(flags=uk.IN_TYPE_BF16 | uk.OUT_TYPE_S8, rows=16, cols=32, M1=1, K1=2, M0=16, K0=16, scale=64, residual=None,
-             total=None, stride=32, eps=1e-5):
-        lib.rmsnorm_pack(64, 0, stride, residual, 0, 32, total, 0, 32, None, eps, 64, 0, 512, scale, rows, cols, M1, K1, M0,
-                         K0, flags)
+             total=None, stride=32, eps=1e-5, src=64, dst=64, total_stride=32, out_stride=512):
+        lib.rmsnorm_pack(src, 0, stride, residual, 0, 32, total, 0, total_stride, None, eps, dst, 0, out_stride, scale, rows,
+                         cols, M1, K1, M0, K0, flags)
 
     bad = [dict(flags=uk.IN_TYPE_BF16), dict(flags=uk.OUT_TYPE_S8), dict(flags=uk.IN_TYPE_BF16 | uk.OUT_TYPE_F16),
            dict(flags=uk.IN_TYPE_F32 | uk.OUT_TYPE_BF16), dict(flags=0x02 | uk.OUT_TYPE_S8),
            dict(flags=uk.IN_TYPE_BF16 | uk.OUT_TYPE_S8 | uk.ACTIVATION_SILU), dict(flags=0x10000 | 0x25),
            dict(rows=17), dict(cols=33), dict(rows=-1), dict(M1=-1), dict(K0=1 << 15), dict(M1=1 << 31),
            dict(M1=1 << 30, M0=16), dict(scale=None), dict(total=64), dict(stride=-32), dict(eps=-1.0),
-           dict(eps=float("nan")), dict(M0=64, K0=128, K1=1)]
+           dict(eps=float("nan")), dict(M0=64, K0=128, K1=1), dict(src=None), dict(dst=None), dict(M1=2, out_stride=511),
+           dict(residual=64, total=64, total_stride=31)]
     for kw in bad:
         with pytest.raises(uk.ContractViolation):
             norm(**kw)
@@ -398,3 +399,39 @@ def test_row_op_refusals(lib):
     for flags in (uk.IN_TYPE_BF16 | uk.OUT_TYPE_S8 | 0x500, uk.IN_TYPE_F16 | uk.OUT_TYPE_F32, 0):
         with pytest.raises(uk.ContractViolation):
             gate(flags)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m0,k0,cols", [(16, 16, 13), (1, 8, 8), (24, 4, 20)])
+def test_more_rows_than_a_launch_takes(lib, m0, k0, cols):
+    """2^21 rows of tiles are a launch: a call of more gives what calls of fewer give, byte by byte."""
+    lib.raise_on_violation(True)
+    rows = (1 << 21) + 1003
+    M1, K1 = -(-rows // m0), -(-cols // k0)
+    panel = K1 * m0 * k0
+    g = torch.Generator(device="cuda").manual_seed(rows + m0)
+    x = torch.randn(rows, cols, generator=g, device="cuda").to(torch.bfloat16)
+    y = torch.randn(rows, cols, generator=g, device="cuda").to(torch.bfloat16)
+    flags = uk.IN_TYPE_BF16 | uk.OUT_TYPE_S8
+    px, py = x.data_ptr(), y.data_ptr()
+
+    def run(part, norm):
+        tiles = torch.full((M1 * panel,), 7, dtype=torch.int8, device="cuda")
+        total = torch.full((rows, cols), 3.0, dtype=torch.bfloat16, device="cuda")
+        scale = torch.full((rows,), 5.0, device="cuda")
+        for m in range(0, M1, part):
+            first, panels = m * m0, min(part, M1 - m)
+            here = min(rows - first, panels * m0)
+            if norm:
+                lib.rmsnorm_pack(px, first * cols, cols, py, first * cols, cols, total.data_ptr(), first * cols, cols, None,
+                                 1e-5, tiles.data_ptr(), m * panel, panel, scale[first:].data_ptr(), here, cols, panels, K1,
+                                 m0, k0, flags)
+            else:
+                lib.gate_pack(px, first * cols, cols, py, first * cols, cols, tiles.data_ptr(), m * panel, panel,
+                              scale[first:].data_ptr(), here, cols, panels, K1, m0, k0, flags | uk.ACTIVATION_SILU)
+        torch.cuda.synchronize()
+        return tiles, total, scale
+
+    for norm in (True, False):
+        for a, b in zip(run(M1, norm), run(100000 // m0, norm)):
+            assert same_bytes(a, b), norm
