@@ -22,9 +22,11 @@ HIP_SOURCES = ["mmt4d_mfma_s16.hip", "mmt4d_mfma_s8s4.hip",
 # kernel instantiations of one pair per object file, built in parallel.
 MFMA_TYPES = {"s8": "kS8", "f16": "kF16", "bf16": "kBF16", "f16f16": "kF16F16",
               "bf16bf16": "kBF16BF16", "f32": "kF32", "f8": "kF8",
-              "s8ep": "kS8Ep", "f16ep": "kF16Ep", "bf16ep": "kBF16Ep", "f8ep": "kF8Ep"}
+              "s8ep": "kS8Ep", "f16ep": "kF16Ep", "bf16ep": "kBF16Ep", "f8ep": "kF8Ep",
+              "f8asf16ep": "kF8AsF16Ep"}
 MFMA_ROW_CLASSES = {"f32": (4, 8, 16), "f8": (16,),
-                    "s8ep": (8, 16), "f16ep": (16,), "bf16ep": (16,), "f8ep": (16,)}
+                    "s8ep": (8, 16), "f16ep": (16,), "bf16ep": (16,), "f8ep": (16,),
+                    "f8asf16ep": (16,)}
 MFMA_INSTANCES = [(t, e, rb) for t, e in MFMA_TYPES.items()
                   for rb in MFMA_ROW_CLASSES.get(t, (2, 4, 8, 16))]
 C_SOURCES = ["uk_host.c", "uk_plugin.c"]

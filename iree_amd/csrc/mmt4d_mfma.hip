@@ -28,6 +28,7 @@ int launch_s8ep_rb16(const Problem& p, int forced, hipStream_t stream, const cha
 int launch_f16ep_rb16(const Problem& p, int forced, hipStream_t stream, const char** name);
 int launch_bf16ep_rb16(const Problem& p, int forced, hipStream_t stream, const char** name);
 int launch_f8ep_rb16(const Problem& p, int forced, hipStream_t stream, const char** name);
+int launch_f8asf16ep_rb16(const Problem& p, int forced, hipStream_t stream, const char** name);
 #undef UK_DECLARE_ROW_CLASSES
 #define UK_DEFINE_BY_ROW_BYTES(T)                                                            \
   inline int launch_##T(const Problem& p, int forced, hipStream_t stream, const char** name) { \
@@ -67,7 +68,10 @@ inline int launch_with_epilogue(Elem e, const Problem& p, hipStream_t stream, co
       return p.rb == 8 ? launch_s8ep_rb8(p, 0, stream, name) : p.rb >= 16 ? launch_s8ep_rb16(p, 0, stream, name) : -1;
     case Elem::kF16: return p.rb >= 16 ? launch_f16ep_rb16(p, 0, stream, name) : -1;
     case Elem::kBF16: return p.rb >= 16 ? launch_bf16ep_rb16(p, 0, stream, name) : -1;
-    case Elem::kF8: return p.rb >= 16 ? launch_f8ep_rb16(p, 0, stream, name) : -1;
+    case Elem::kF8:
+      return p.rb < 16             ? -1
+             : p.ep.out_bytes == 4 ? launch_f8asf16ep_rb16(p, 0, stream, name)
+                                   : launch_f8ep_rb16(p, 0, stream, name);
     default: return -1;
   }
 }

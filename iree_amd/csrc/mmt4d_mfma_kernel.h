@@ -90,11 +90,12 @@ typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 // pipeline only (PIPE 5 below, which describes the arithmetic).
 // k...Ep: the same operands and sums, whose results go through an epilogue
 // (mmt4d_mfma_epilogue.h) into a row-major matrix.
-enum class Elem { kS8, kF16, kBF16, kF8, kF32, kF16F16, kBF16BF16, kS8S4, kS16, kS8Ep, kF16Ep, kBF16Ep, kF8Ep, kS8S4Ep };
+enum class Elem { kS8, kF16, kBF16, kF8, kF32, kF16F16, kBF16BF16, kS8S4, kS16, kS8Ep, kF16Ep, kBF16Ep, kF8Ep, kF8AsF16Ep, kS8S4Ep };
 
 template <Elem E>
 constexpr bool has_epilogue() {
-  return E == Elem::kS8Ep || E == Elem::kF16Ep || E == Elem::kBF16Ep || E == Elem::kF8Ep || E == Elem::kS8S4Ep;
+  return E == Elem::kS8Ep || E == Elem::kF16Ep || E == Elem::kBF16Ep || E == Elem::kF8Ep ||
+         E == Elem::kF8AsF16Ep || E == Elem::kS8S4Ep;
 }
 
 typedef uint16_t v4u16 __attribute__((ext_vector_type(4)));
@@ -234,6 +235,32 @@ template <> struct ElemTraits<Elem::kS8Ep> : ElemTraits<Elem::kS8> {};
 template <> struct ElemTraits<Elem::kF16Ep> : ElemTraits<Elem::kF16> {};
 template <> struct ElemTraits<Elem::kBF16Ep> : ElemTraits<Elem::kBF16> {};
 template <> struct ElemTraits<Elem::kF8Ep> : ElemTraits<Elem::kF8> {};
+// 8-bit floats whose sums keep f32: the 8-bit instructions cut the products off at bits of the
+// largest of them (both forms are 1.3e-5 of the root mean square off for normal operands, at any
+// K), which f16's, with the same values, do not (6e-8 at K = 2176). A matrix of 16 bits does not
+// tell the two apart (its own half step is 2.4e-4 and more); one of f32 does. us into bf16 by the 8-bit
+// instructions / into f32 by these: 1 x 28672 x 8192 38.2 / 41.6, 512 x 8192 x 8192 43.6 / 82.3, 4096^3
+// 60.9 / 169 (812 TFLOP/s, bound by f16's rate and the conversions of fragments).
+template <> struct ElemTraits<Elem::kF8AsF16Ep> {
+  using Acc = v4f;
+  using Out = Out32<v4f, float>;
+  static constexpr int kHalves = 2;
+  static __device__ __forceinline__ v8h widened(int lo, int hi) {
+    typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+    const v2h x0 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, false);
+    const v2h x1 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, true);
+    const v2h x2 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, false);
+    const v2h x3 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, true);
+    return v8h{x0[0], x0[1], x1[0], x1[1], x2[0], x2[1], x3[0], x3[1]};
+  }
+  static __device__ __forceinline__ Acc mfma(const v4i* a, const v4i* b, Acc c) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      c = __builtin_amdgcn_mfma_f32_16x16x32_f16(widened(a[i / 2][i % 2 * 2], a[i / 2][i % 2 * 2 + 1]),
+                                                 widened(b[i / 2][i % 2 * 2], b[i / 2][i % 2 * 2 + 1]), c, 0, 0, 0);
+    return c;
+  }
+};
 template <> struct ElemTraits<Elem::kS8S4Ep> : ElemTraits<Elem::kS8S4> {};
 
 // LDS-direct loads (PIPE 5): address-space-qualified pointers for the builtin,

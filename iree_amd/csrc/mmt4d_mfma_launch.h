@@ -1057,6 +1057,10 @@ int launch_class(const Problem& p, int forced, hipStream_t stream, const char** 
   // a unit, overlap their prologues and stores (s8 16x16x2 7070 x 2547 x 16: 21.9
   // us in 256x256 blocks, 17.5 in 128x128).
   if (forced == 0 && (choice == 1 || choice == 7) && ((int64_t)p.K1 << p.lrb) < BIG_KS) choice = 2;
+  // Fragments that are widened take four times their registers: blocks of 256 rows would
+  // have 84 to 284 bytes a lane of them in scratch memory.
+  constexpr bool kBigBlocks = E != Elem::kF8AsF16Ep;
+  if (!kBigBlocks && (choice == 1 || choice == 7)) choice = 2;
   if (choice == 1 && forced == 0) {
     // Tile quantization: a last row or column of 256x256 workgroups that is
     // mostly padding can cost a whole extra round on the 256 CUs. Compare, in
@@ -1223,7 +1227,7 @@ int launch_class(const Problem& p, int forced, hipStream_t stream, const char** 
         if (st > 0) return st;
       }
     }
-    if constexpr (RBC >= 16) {
+    if constexpr (RBC >= 16 && kBigBlocks) {
       // Both operands through LDS-direct loads, two wave groups alternating
       // between memory and compute phases (PIPE 5 of mmt4d_mfma_kernel.h): the
       // default for the big problems of the 8- and 16-bit types (s8 8192^3
@@ -1299,7 +1303,7 @@ int launch_class(const Problem& p, int forced, hipStream_t stream, const char** 
     // 256 rows x 128 columns, 8 waves of 128x32: for problems with too few
     // 256x256 blocks to fill the CUs; moves fewer L1 bytes per MFMA than the
     // 128x128 shape.
-    if constexpr (RBC >= 16) {
+    if constexpr (RBC >= 16 && kBigBlocks) {
       if (forced == 20 || (forced == 0 && E != Elem::kF32)) {
         int st = launch_variant<E, RBC, 8, 2, 2, 4, 1, 5>(p, 0, p.K1, p.accumulate, stream);
         if (st == 0) *name = "mmt4d_mfma_256x128_lds_direct";
@@ -1315,7 +1319,7 @@ int launch_class(const Problem& p, int forced, hipStream_t stream, const char** 
   }
   // (With 24 KB of K and more the 64x64 blocks below split K over workgroups.)
   const bool long_k = ((int64_t)p.K1 << p.lrb) >= 24576;
-  if constexpr (RBC >= 8 && E != Elem::kF32) {
+  if constexpr (RBC >= 8 && E != Elem::kF32 && E != Elem::kF8AsF16Ep) {
     if (choice == 6 && (forced == 21 || (forced == 0 && k_slices_override() == 0))) {
       const int slices = forced == 21 ? k_slices_override() : slices_that_pay<E, RBC>(p, rows_m, cols_n, long_k);
       const int st = launch_slices<E, RBC>(p, slices, stream);

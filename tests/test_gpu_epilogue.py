@@ -274,3 +274,37 @@ def test_epilogue_refusals(lib):
     call(rows=0)
     call(cols=0)
     call(rows=0, M=0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type_,K0", [(F8, 32), (F8, 16), (F16, 8), (BF16, 8)])
+def test_f32_matrices_have_sums_in_f32(gpu, type_, K0):
+    """Operands whose products spread over many binades: the sums keep f32. K additions, each rounded by
+    up to 2^-24 of a sum that is no larger (in the root mean square) than the last one, and independently of
+    one another, are off by sqrt(K) 2^-24 of it; by twice that if an instruction cuts off what others round.
+    At K = 1000 that is 3.8e-6, where products that have lost their low bits are 1.3e-5 off."""
+    lib, _ = gpu
+    g = torch.Generator().manual_seed(5)
+    names = set()
+    for rows, cols, k in [(1, 300, 1000), (12, 109, 700), (40, 150, 333), (300, 300, 1000), (1000, 1100, 1000), (2100, 2100, 512)]:
+        M0 = 1 if rows == 1 else 16
+        M1, N1, K1 = -(-rows // M0), -(-cols // 16), -(-k // K0)
+
+        def operand(n, t0, t1):
+            full = torch.zeros(t1 * t0, K1 * K0)
+            full[:n, :k] = 40 * torch.randn(n, k, generator=g)
+            full = full.to(TORCH[type_])
+            tiles = full.view(torch.int8 if type_ == F8 else torch.int16).view(t1, t0, K1, K0).transpose(1, 2).contiguous()
+            return tiles.cuda(), full[:n].double()
+
+        (lhs, a), (rhs, b) = operand(rows, M0, M1), operand(cols, 16, N1)
+        out = torch.empty(rows, cols, device="cuda")
+        lib.mmt4d_epilogue_unpack(lhs.data_ptr(), 0, lhs[0].numel(), rhs.data_ptr(), 0, rhs[0].numel(), None, 0, 0,
+                                  out.data_ptr(), 0, cols, rows, cols, None, None, None, M1, N1, K1, M0, 16, K0, type_,
+                                  uk.OUT_TYPE_F32)
+        lib.synchronize()
+        names.add(lib.last_kernel_name())
+        want = a @ b.T
+        off = ((out.cpu().double() - want).norm() / want.norm()).item()
+        assert off <= 2 * k ** 0.5 * U32, (rows, cols, k, off, lib.last_kernel_name())
+    assert len(names) >= 3, names
