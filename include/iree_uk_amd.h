@@ -761,7 +761,8 @@ enum {
   IREE_UK_AMD_FLAG_OUT_TYPE_F8E4M3FN = 0x80,
   /* Activation:  NONE  x;  RELU  x < 0 ? 0 : x;  SILU  x / (1 + e^-x);
    *   GELU       x/2 * (1 + erf(x / sqrt 2));
-   *   GELU_TANH  x/2 * (1 + tanh(sqrt(2/pi) * (x + 0.044715 x^3))). */
+   *   GELU_TANH  x/2 * (1 + tanh(sqrt(2/pi) * (x + 0.044715 x^3))).
+   * The lowest numbers give zero, -infinity zero (RELU, GELU) or NaN. */
   IREE_UK_AMD_FLAG_ACTIVATION_MASK = 0xF00,
   IREE_UK_AMD_FLAG_ACTIVATION_NONE = 0x000,
   IREE_UK_AMD_FLAG_ACTIVATION_RELU = 0x100,

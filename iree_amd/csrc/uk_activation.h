@@ -26,14 +26,16 @@ __device__ __forceinline__ float times_sigmoid(float x, float t) {
 // e^-t = 2^hi e^lo with lo = -t - hi ln 2, and e^lo = 1 + lo. (f8 2000 x 5001 with SILU: 9
 // elements beside the 64-bit result's, 10 with correctly rounded steps; times_sigmoid has twice
 // as many, and gate_pack takes 14.5 us with it, so 16.0, with a Newton step behind the
-// reciprocal, too, 16.7.) Beyond 126 ln 2 the sigmoid is no normal f32 any more.
+// reciprocal, too, 16.7.) Beyond 126 ln 2 the sigmoid is no normal f32 any more: below that it is
+// zero, also times the lowest numbers, which masks are made of.
 __device__ __forceinline__ float times_sigmoid_close(float x, float t) {
   constexpr float kLog2e = 1.44269502f, kLn2 = 0.693147182f, kMost = 87.3365448f;
+  const bool none = t < -kMost;
   t = __builtin_amdgcn_fmed3f(t, -kMost, kMost);
   const float hi = -kLog2e * t;
   const float lo = __builtin_fmaf(-kLn2, hi, -t);
   const float e = __builtin_amdgcn_exp2f(hi);
-  return x * __builtin_amdgcn_rcpf(__builtin_fmaf(e, lo, 1.0f + e));
+  return x * (none ? 0.0f : __builtin_amdgcn_rcpf(__builtin_fmaf(e, lo, 1.0f + e)));
 }
 
 // x Phi(x) with Phi(x) = erfc(-x / sqrt 2) / 2. With s = |x| and tail = s erfc(s / sqrt 2) / 2

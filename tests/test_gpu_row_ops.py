@@ -435,3 +435,70 @@ def test_more_rows_than_a_launch_takes(lib, m0, k0, cols):
     for norm in (True, False):
         for a, b in zip(run(M1, norm), run(100000 // m0, norm)):
             assert same_bytes(a, b), norm
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tin", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("cols", [100, 70001])
+def test_gates_of_the_lowest_numbers_are_zero(gpu, tin, cols):
+    """What a mask puts into a gate: every activation makes zeros of it, and the row's scale is that of its other columns.
+    -infinity: zero, or NaN where the formula multiplies it by zero."""
+    lib, _ = gpu
+    dt, fin, fout = TYPES[tin]
+    low = torch.finfo(dt).min
+    g = torch.Generator().manual_seed(3)
+    gate = torch.randn(4, cols, generator=g).to(dt)
+    gate[0, 1::3] = low
+    gate[1, :] = low
+    gate[2, 5] = low / 4
+    gate[2, 7] = -60000.0
+    gate[3, 2] = -float("inf")
+    masked = [gate[0] == low, gate[1] == low, gate[2] < -1000]
+    up = torch.randn(4, cols, generator=g).to(dt).cuda()
+    K1 = -(-cols // 16)
+    x = gate.cuda()
+    for act in ("relu", "gelu", "gelu_tanh", "silu"):
+        kept = act64(gate.double().numpy()[:3], act) * up[:3].cpu().double().numpy()
+        top = np.abs(np.where(torch.stack(masked).numpy(), 0.0, kept)).max(axis=1)
+        for tout, fo in ((tin, fout), ("s8", uk.OUT_TYPE_S8)):
+            tiles = torch.zeros(K1 * 16 * 4, dtype=torch.int8 if tout == "s8" else dt, device="cuda")
+            scale = torch.zeros(4, device="cuda")
+            lib.gate_pack(x.data_ptr(), 0, cols, up.data_ptr(), 0, cols, tiles.data_ptr(), 0, K1 * 16, scale.data_ptr(), 4, cols,
+                          4, K1, 1, 16, fin | fo | ACTS[act])
+            lib.synchronize()
+            got = tiles.cpu().double().view(4, K1 * 16)[:, :cols]
+            for row, m in enumerate(masked):
+                assert not got[row][m].any(), (act, tout, row)
+            assert got[0][~masked[0]].any() and got[2].any() and not got[:3].isnan().any(), (act, tout)
+            limit = act in ("relu", "gelu")
+            if tout == "s8":
+                # (1e-5: the activation's own 2e-6 at most, and the scale's roundings)
+                assert np.allclose(scale[:3].cpu().numpy(), top / 127, rtol=1e-5, atol=0), (act, scale, top / 127)
+                assert scale[3].isnan().item() != limit and got[3].any().item() == limit
+            else:
+                assert got[3, 2].isnan().item() != limit and (not limit or got[3, 2] == 0)
+
+
+@pytest.mark.gpu
+def test_epilogues_of_the_lowest_numbers_are_zero(gpu):
+    """A bias of the lowest number masks a column: zeros, with every activation, beside a residual, too."""
+    lib, _ = gpu
+    a = torch.ones(2, 4, 16, 16, dtype=torch.int8, device="cuda")
+    b = torch.ones(3, 4, 16, 16, dtype=torch.int8, device="cuda")
+    bias = torch.zeros(48, device="cuda")
+    bias[7] = torch.finfo(torch.float32).min
+    bias[40] = -1e30
+    for act in ("relu", "gelu", "gelu_tanh", "silu"):
+        for mode in (uk.KERNEL_MODE_AUTO, uk.KERNEL_MODE_GENERIC):
+            lib.set_kernel_mode(mode)
+            try:
+                out = torch.full((32, 48), 2.0, device="cuda")
+                lib.mmt4d_epilogue_unpack(a.data_ptr(), 0, a.stride(0), b.data_ptr(), 0, b.stride(0), out.data_ptr(), 0, 48,
+                                          out.data_ptr(), 0, 48, 32, 48, None, None, bias.data_ptr(), 2, 3, 4, 16, 16, 16,
+                                          uk.MMT4D_TYPE_S8S8S32, uk.OUT_TYPE_F32 | ACTS[act])
+                lib.synchronize()
+            finally:
+                lib.set_kernel_mode(uk.KERNEL_MODE_AUTO)
+            other = torch.ones(48, dtype=torch.bool)
+            other[7] = other[40] = False
+            assert bool((out[:, 7] == 2).all()) and bool((out[:, 40] == 2).all()) and bool((out.cpu()[:, other] == 66).all()), act
