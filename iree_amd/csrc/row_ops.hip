@@ -72,7 +72,7 @@ __device__ __forceinline__ void eight_bit_scale(float top, float r, float& scale
 // and what is stored comes out of registers.
 //
 // Bound by memory, with every byte moved once (measured: norm 2048 x 8192 bf16 into f8 reads
-// 67 MB and writes 49, gate 2048 x 28672 235 and 58): 26.2 us (4.5 TB/s) and 66.0 us (4.4 TB/s),
+// 67 MB and writes 49, gate 2048 x 28672 235 and 58): 26.2 us (4.5 TB/s) and 63.5 us (4.6 TB/s),
 // where a copy of 1 GiB by torch moves 4.8 TB/s, by the best of the kernels tried 5.8. The
 // vector ALU is busy for over half of the gate's time (the exponential and the reciprocal of
 // SILU). Small calls are the launch and one round trip: norm 1 x 4096 4.6 us, pack of as many
@@ -197,7 +197,7 @@ __global__ __launch_bounds__(kMaxThreads) void row_op_kernel(RowArgs a) {
       const int c = first + i * step, k = i % P;
       if (k == 0) {
 #pragma unroll
-        for (int j = 0; j < P; ++j) {
+        for (int j = 0; j < P && i + j < C; ++j) {
           x[j].load(in, c + j * step, row_bytes);
           if (a.second) y[j].load(second, c + j * step, row_bytes);
           if (NORM && a.weight) z[j].load(a.weight, c + j * step, row_bytes);
@@ -480,10 +480,14 @@ extern "C" int iree_uk_amd_hip_launch_row_op(const iree_uk_amd_row_op_t* p, void
     constexpr bool N = decltype(norm)::value;
     constexpr Form F = decltype(form_c)::value;
     using IN = decltype(in_type);
-    auto kernel = each <= 1   ? row_op_kernel<N, IN, F, 1>
-                  : each <= 2 ? row_op_kernel<N, IN, F, 2>
-                  : each <= 4 ? row_op_kernel<N, IN, F, 4>
-                              : row_op_kernel<N, IN, F, N ? 4 : 8>;
+    // (An instance for every number of chunks: with powers of two alone gate 2048 x 11008 took
+    // 29.6 us, so 26.2, 2048 x 28672 66.3 and 63.5, norm 2048 x 12288 38.5 and 37.0.)
+    using Kernel = void (*)(RowArgs);
+    static constexpr Kernel by_chunks[8] = {
+        row_op_kernel<N, IN, F, 1>,         row_op_kernel<N, IN, F, 2>,         row_op_kernel<N, IN, F, 3>,
+        row_op_kernel<N, IN, F, 4>,         row_op_kernel<N, IN, F, N ? 4 : 5>, row_op_kernel<N, IN, F, N ? 4 : 6>,
+        row_op_kernel<N, IN, F, N ? 4 : 7>, row_op_kernel<N, IN, F, N ? 4 : 8>};
+    const Kernel kernel = by_chunks[in_registers && each > 1 ? each - 1 : 0];
     // A grid has fewer than 2^32 threads: whole tiles of up to 2^21 rows a launch (a tile
     // has 4096 bytes at most, so 4096 rows).
     const int64_t most_panels = (1ll << 21) / p->M0;
