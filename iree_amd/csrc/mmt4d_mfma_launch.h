@@ -568,6 +568,9 @@ inline int finish_k(int st) { return st < 0 ? (int)hipErrorUnknown : st; }
 // that adds them up (mmt4d_mfma_sum.h). Returns a HIP status, or -1 where K is no
 // whole number of steps, `slices` are too many for it, or there is no workspace (a
 // stream under capture, iree_uk_amd_mmt4d_no_alloc with a large result).
+// In front of an epilogue K may end inside a step: that end is one more slice, of a launch
+// of its own (f8 577 x 1716 x 25695 119.6 us in 64x64 blocks, so 55.8; bf16 577 x 1716 x 13001 132.0 and
+// 54.8; s8 1000 x 1000 x 25695 61.9 and 45.7).
 template <Elem E, int RBC>
 int launch_slices(const Problem& p, int slices, hipStream_t stream) {
   // 16-bit results: the sums of the slices are 32-bit floats like those of a block.
@@ -580,14 +583,16 @@ int launch_slices(const Problem& p, int slices, hipStream_t stream) {
   constexpr int KS = 64 * ElemTraits<E>::kHalves;
   const int64_t k_bytes = (int64_t)p.K1 << p.lrb;
   if (p.out_rows <= 0 || p.out_cols <= 0) return 0;
-  if (k_bytes % KS || slices < 2 || k_bytes / KS < 16 * slices) return -1;
+  const int32_t rest = (int32_t)(k_bytes % KS >> p.lrb);   // K-tiles
+  if ((rest && !has_epilogue<E>()) || slices < 2 || k_bytes / KS < 16 * slices) return -1;
+  const int parts = slices + (rest > 0);
   const int64_t rows = (int64_t)p.M1 * p.M0, cols = (int64_t)p.N1 * p.N0;
   if (p.out_sm0 >= (1ll << 32) || p.out_spn >= (1ll << 32) || p.acc_sm0 >= (1ll << 32) ||
-      p.acc_spn >= (1ll << 32) || rows * cols * slices >= (1ll << 26)) {
+      p.acc_spn >= (1ll << 32) || rows * cols * parts >= (1ll << 26)) {
     return -1;
   }
   KSplitWorkspace ws{};
-  const int got = acquire_ksplit_workspace((size_t)(slices * rows * cols) * 4, 1, stream, &ws);
+  const int got = acquire_ksplit_workspace((size_t)(parts * rows * cols) * 4, 1, stream, &ws);
   if (got != 0) return got > 1 ? got : -1;
   Problem q = p;
   q.out = ws.partials;
@@ -600,14 +605,22 @@ int launch_slices(const Problem& p, int slices, hipStream_t stream) {
   q.out_rows = std::min(p.out_rows, rows);
   q.out_cols = std::min(p.out_cols, cols);
   q.accumulate = q.dequant = false;
-  int st = launch_variant<P, RBC, 4, 2, 2, 4, 1, 5, true>(q, 0, q.K1, false, stream, slices);
+  int st = launch_variant<P, RBC, 4, 2, 2, 4, 1, 5, true>(q, 0, q.K1 - rest, false, stream, slices);
   if (st != 0) return st;
+  if constexpr (has_epilogue<E>()) {
+    if (rest) {
+      q.out += slices * rows * cols * 4;
+      q.acc = q.out;
+      st = launch_variant<P, RBC, 4, 2, 2, 4, 1, 5>(q, q.K1 - rest, rest, false, stream);
+      if (st != 0) return st;
+    }
+  }
   note_k_slices(slices);
   SumArgs s{};
   s.partials = ws.partials;
   s.slice_bytes = rows * cols * 4;
   s.pitch = cols * 4;
-  s.slices = slices;
+  s.slices = parts;
   s.rows = (int32_t)std::min(rows, p.out_rows);
   s.cols = (int32_t)std::min(cols, p.out_cols);
   s.M0 = p.M0; s.N0 = p.N0;
@@ -945,7 +958,8 @@ int slices_that_pay(const Problem& p, int64_t rows, int64_t cols, bool long_k) {
   const int64_t slices = std::min<int64_t>(std::min<int64_t>(cus / b128, 16), k_bytes / least_k);
   if (slices < 2) return 0;
   const double kb = (double)k_bytes / 1024;
-  const double here = 5 + 4.3 * kb / (double)slices + 2.4e-6 * (double)(slices * rows * cols);
+  const bool rest = has_epilogue<E>() && k_bytes % (64 * ElemTraits<E>::kHalves) != 0;   // (a launch more)
+  const double here = (rest ? 9 : 5) + 4.3 * kb / (double)slices + 2.4e-6 * (double)(slices * rows * cols);
   const double units = (double)b64 / (double)cus;
   double blocks = 2 + (RBC == 8 ? 2.8 : 2.05) * kb * std::max(1.0, std::min(std::ceil(units), units + 0.3));
   if (!long_k && b32 <= 2 * cus) blocks = 2 + 0.9 * kb * (double)uk::ceil_div(b32, cus);

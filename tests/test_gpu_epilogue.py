@@ -308,3 +308,16 @@ def test_f32_matrices_have_sums_in_f32(gpu, type_, K0):
         off = ((out.cpu().double() - want).norm() / want.norm()).item()
         assert off <= 2 * k ** 0.5 * U32, (rows, cols, k, off, lib.last_kernel_name())
     assert len(names) >= 3, names
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type_,M0,K0", [(S8, 16, 16), (S8, 32, 8), (F8, 1, 32), (F16, 16, 8), (BF16, 1, 8)])
+def test_slices_of_a_k_that_ends_inside_a_step(gpu, type_, M0, K0):
+    """K in slices and what is left of it as one more, with a residual and without, row-major and at odd pitches."""
+    lib, _ = gpu
+    names = set()
+    for rows, cols, k, residual, pitch in [(577, 716, 9001, "own", 0), (400, 1000, 12309, "in place", 3),
+                                           (1000, 999, 16001, None, 1), (577, 716, 8968, "own", 5)]:
+        for out in ("f32", "bf16"):
+            names.add(run(lib, type_, rows, cols, k, M0, 16, K0, out, "silu", residual=residual, pitch=pitch, offset=pitch))
+    assert any("kslices" in n for n in names), names
