@@ -952,8 +952,14 @@ int slices_that_pay(const Problem& p, int64_t rows, int64_t cols, bool long_k) {
   const int64_t b64 = workgroups(p, 64, 64);
   const int64_t b32 = uk::ceil_div(rows, (int64_t)32) * uk::ceil_div(cols, (int64_t)32);
   const int64_t b16 = uk::ceil_div(rows, (int64_t)16) * uk::ceil_div(cols, (int64_t)16);
-  // (With fewer than 32 64x64 blocks K is in more parts there than it would be here.)
-  if (cus < 1 || b128 < 1 || b64 < 32 || b16 <= cus) return 0;
+  // (With fewer than 32 64x64 blocks K is in more parts there than it would be here. In front of
+  // an epilogue slices are ahead all the same from 24 KB of K on: the workgroup that arrives last
+  // there reads the parts one after the other, 1.15 us each, and finishes its block alone. us there /
+  // here with s8 100 x 300 x 24576 43.8 / 13.5, 300 x 300 x 65536 42.3 / 22.2, f8 65 x 65 x 24576 26.2 /
+  // 15.8, bf16 200 x 200 x 16384 34.6 / 15.6.)
+  if (cus < 1 || b128 < 1) return 0;
+  const bool few = b64 < 32 || b16 <= cus;
+  if (few && !(has_epilogue<E>() && long_k)) return 0;
   const int64_t least_k = long_k && ElemTraits<E>::kHalves == 1 ? 1536 : 2048;
   const int64_t slices = std::min<int64_t>(std::min<int64_t>(cus / b128, 16), k_bytes / least_k);
   if (slices < 2) return 0;
@@ -963,7 +969,10 @@ int slices_that_pay(const Problem& p, int64_t rows, int64_t cols, bool long_k) {
   const double units = (double)b64 / (double)cus;
   double blocks = 2 + (RBC == 8 ? 2.8 : 2.05) * kb * std::max(1.0, std::min(std::ceil(units), units + 0.3));
   if (!long_k && b32 <= 2 * cus) blocks = 2 + 0.9 * kb * (double)uk::ceil_div(b32, cus);
-  else if (long_k && 2 * b64 <= cus) blocks = 15 + 2.05 * kb / (double)(cus / b64);
+  else if (long_k && 2 * b64 <= cus) {
+    const double parts = (double)std::min<int64_t>(cus / b64, 32);
+    blocks = 15 + 2.05 * kb / parts + (has_epilogue<E>() ? 1.15 * parts : 0.0);
+  }
   return here < blocks ? (int)slices : 0;
 }
 
