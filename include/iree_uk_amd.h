@@ -906,8 +906,8 @@ IREE_UK_AMD_EXPORT void iree_uk_amd_gate_pack_p(
  * which a 16-bit matrix does not show: f8 into f32 multiplies the same values
  * as f16 instead, at half the rate and less.
  *
- * One launch, and no memory beyond the operands but what iree_uk_mmt4d keeps for
- * the same product, for s8 (tile rows of 8 bytes and more), f16, bf16 and f8 (16
+ * One launch, and no memory beyond the operands but a workspace like iree_uk_mmt4d's
+ * for sums in parts of K (with a launch or two more; up to 75 MB), for s8 (tile rows of 8 bytes and more), f16, bf16 and f8 (16
  * bytes and more, what iree_uk_query_tile_sizes_2d answers with) and s8 x s4.
  * Other types and tile rows run as a product into f32 and an epilogue of its
  * own, in place for an f32 matrix, else from a buffer that the library keeps per

@@ -961,11 +961,22 @@ int slices_that_pay(const Problem& p, int64_t rows, int64_t cols, bool long_k) {
   const bool few = b64 < 32 || b16 <= cus;
   if (few && !(has_epilogue<E>() && long_k)) return 0;
   const int64_t least_k = long_k && ElemTraits<E>::kHalves == 1 ? 1536 : 2048;
-  const int64_t slices = std::min<int64_t>(std::min<int64_t>(cus / b128, 16), k_bytes / least_k);
-  if (slices < 2) return 0;
+  const int64_t most = std::min<int64_t>(16, k_bytes / least_k);
+  int64_t slices = std::min<int64_t>(cus / b128, most);
   const double kb = (double)k_bytes / 1024;
   const bool rest = has_epilogue<E>() && k_bytes % (64 * ElemTraits<E>::kHalves) != 0;   // (a launch more)
-  const double here = (rest ? 9 : 5) + 4.3 * kb / (double)slices + 2.4e-6 * (double)(slices * rows * cols);
+  auto cost = [&](int64_t n) {
+    return (rest ? 9 : 5) + 4.3 * kb / (double)n * (double)uk::ceil_div(n * b128, cus) + 2.4e-6 * (double)(n * rows * cols);
+  };
+  // In front of an epilogue blocks that fill more than half of the units have slices in several
+  // rounds (us in 64x64 blocks / here: s8 1500 x 1500 x 28672 128.7 / 93.7, 700 x 3000 x 25695 149.3 / 92.6,
+  // bf16 1600 x 1600 x 12288 105.6 / 85.1); five at most, whose sums take 63 MB of the workspace.
+  if (has_epilogue<E>() && long_k && slices < 2) {
+    for (int64_t n = 2; n <= std::min<int64_t>(most, 5); ++n)
+      if (slices < 2 || cost(n) < cost(slices)) slices = n;
+  }
+  if (slices < 2) return 0;
+  const double here = cost(slices);
   const double units = (double)b64 / (double)cus;
   double blocks = 2 + (RBC == 8 ? 2.8 : 2.05) * kb * std::max(1.0, std::min(std::ceil(units), units + 0.3));
   if (!long_k && b32 <= 2 * cus) blocks = 2 + 0.9 * kb * (double)uk::ceil_div(b32, cus);

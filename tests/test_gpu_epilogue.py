@@ -321,3 +321,16 @@ def test_slices_of_a_k_that_ends_inside_a_step(gpu, type_, M0, K0):
         for out in ("f32", "bf16"):
             names.add(run(lib, type_, rows, cols, k, M0, 16, K0, out, "silu", residual=residual, pitch=pitch, offset=pitch))
     assert any("kslices" in n for n in names), names
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type_,rows,cols,k", [(BF16, 700, 1700, 12309), (BF16, 700, 1700, 12288), (S8, 100, 300, 24700),
+                                               (F8, 65, 65, 24576), (S8, 1700, 1300, 24600), (F8, 300, 300, 25695)])
+def test_slices_of_a_long_k(gpu, type_, rows, cols, k):
+    """From 24 KB of K on, few blocks and such as fill more than half of the units have K in slices."""
+    lib, _ = gpu
+    K0 = 8 if type_ == BF16 else 16
+    names = set()
+    for i, out in enumerate(("f32", "bf16")):
+        names.add(run(lib, type_, rows, cols, k, 16, 16, K0, out, "silu", residual="own", pitch=i, offset=i))
+    assert any("kslices" in n for n in names), names
