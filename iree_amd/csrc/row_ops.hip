@@ -279,7 +279,7 @@ __global__ __launch_bounds__(kMaxThreads) void row_op_kernel(RowArgs a) {
   if (!tiled) return;
   float r = 1.0f;
   if constexpr (NORM) r = reciprocal_norm(total, a.cols, a.epsilon);
-  float factor = r;
+  float factor = exists ? r : 0.0f;   // (a row beyond the matrix has no sum of squares, and r may be infinite)
   if constexpr (FORM != Form::kSame) {
     float scale;
     eight_bit_scale<FORM>(__uint_as_float(largest), r, scale, factor);
@@ -303,6 +303,14 @@ __global__ __launch_bounds__(kMaxThreads) void row_op_kernel(RowArgs a) {
     uint32_t w[kChunk * OB / 4];
 #pragma unroll
     for (int e = 0; e < kChunk; ++e) u[i][e] *= factor;
+    if constexpr (NORM && FORM == Form::kSame) {
+      // A row that has no norm is NaN, and zero times that: not so the columns beyond it.
+      if (!(factor < __builtin_inff())) {
+#pragma unroll
+        for (int e = 0; e < kChunk; ++e)
+          if (c + e >= a.cols) u[i][e] = 0.0f;
+      }
+    }
     if constexpr (FORM == Form::kS8) {
       // Adding 1.5 * 2^23 rounds to an integer, whose low bits are the sum's.
 #pragma unroll

@@ -502,3 +502,26 @@ def test_epilogues_of_the_lowest_numbers_are_zero(gpu):
             other = torch.ones(48, dtype=torch.bool)
             other[7] = other[40] = False
             assert bool((out[:, 7] == 2).all()) and bool((out[:, 40] == 2).all()) and bool((out.cpu()[:, other] == 66).all()), act
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tin", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("cols", [5, 65, 4093, 32769])
+def test_norm_padding_is_zero_whatever_the_rows_hold(gpu, tin, cols):
+    """Into the in type: rows of tiles beyond the matrix and columns beyond a row are zeros also where nothing is added to
+    the mean of squares, and beside rows that have no norm; those are NaN themselves. Rows in registers and longer ones."""
+    lib, _ = gpu
+    x = np.random.default_rng(cols).standard_normal((6, cols))
+    x[1] = 0
+    x[2, cols // 2] = np.nan
+    x[3, cols - 1] = -np.inf
+    x[4] = 1e30   # (f16: infinity)
+    for eps in (0.0, 1e-5):
+        y, slack, tiles, _, name = run_norm(lib, tin, tin, 6, cols, 8, 16, residual=False, with_sum=False, weight=True,
+                                            values=x, M1=2, K1=-(-cols // 16) + 2, eps=eps)
+        got = tiles_to_matrix(tiles)
+        assert not got[6:].any() and not got[:, cols:].any(), name
+        assert np.isnan(got[2:5, :cols]).all(), name
+        assert np.isnan(got[1, :cols]).all() if eps == 0 else not got[1].any(), name
+        keep = [0, 5]
+        check_rows(y[keep], slack[keep], tin, tin, tiles[:1][:, :, keep, :], None, 2, cols, name)
