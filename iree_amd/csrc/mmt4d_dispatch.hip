@@ -90,10 +90,31 @@ bool overlaps(const char* a, int64_t a_bytes, const char* b, int64_t b_bytes) {
   return a < b + b_bytes && b < a + a_bytes;
 }
 
+// The scaled product of 8-bit floats in f32, in tile rows of any width: by the kernels that end
+// in an epilogue (here one that adds nothing), which multiply as f16 what goes into an f32
+// matrix; rows under 16 bytes are regrouped first. The other kernels for 8-bit floats lose bits
+// that such a matrix shows: 1.5e-5 of the root mean square off, these 3e-8 (300 x 300 x 1000 in
+// rows of 8 bytes). Returns a HIP status.
+int launch_f8_into_f32(const iree_uk_mmt4d_params_t* p, const iree_uk_amd_rowmajor_out_t* rm, void* stream,
+                       int kernel_mode, const char** kernel_name) {
+  iree_uk_amd_rowmajor_out_t r = *rm;
+  r.epilogue = 1;
+  r.epilogue_flags = IREE_UK_AMD_FLAG_OUT_TYPE_F32 | IREE_UK_AMD_FLAG_ACTIVATION_NONE;
+  r.bias = nullptr;
+  r.residual = nullptr;
+  int st = iree_uk_amd_hip_launch_mmt4d_mfma(p, &r, stream, 0, kernel_name);
+  if (st < 0 && kernel_mode == IREE_UK_AMD_KERNEL_MODE_AUTO)
+    st = iree_uk_amd_hip_launch_mmt4d_retiled(p, &r, stream, kernel_name);
+  if (st >= 0) return st;
+  *kernel_name = "mmt4d_generic";
+  return iree_uk_amd_hip_launch_mmt4d_generic(p, &r, stream);
+}
+
 // Types and tiles that have no kernel with an epilogue of its own (mmt4d_mfma.hip): the
-// product into f32 with its scales, on whatever kernel serves it, and the epilogue as a
-// second launch; in place where the matrix is f32 and its residual another one, else from
-// a buffer. Returns a HIP status, or -1 where there is no buffer to be had.
+// product into f32 with its scales, on whatever kernel serves it (8-bit floats into f32: one
+// that keeps their bits), and the epilogue as a second launch; in place where the matrix is f32
+// and its residual another one, else from a buffer. Returns a HIP status, or -1 where there is
+// no buffer to be had.
 int launch_epilogue_apart(const iree_uk_mmt4d_params_t* p, const iree_uk_amd_rowmajor_out_t* rm, void* stream,
                           int kernel_mode, const char** kernel_name) {
   ApartArgs a{};
@@ -108,6 +129,8 @@ int launch_epilogue_apart(const iree_uk_mmt4d_params_t* p, const iree_uk_amd_row
                         !(rm->residual && overlaps((const char*)p->out_buffer, (rm->size0 - 1) * a.ep.out_pitch + row_bytes,
                                                    (const char*)rm->residual,
                                                    (rm->size0 - 1) * a.ep.residual_pitch + row_bytes));
+  const bool f8_into_f32 = (p->flags & IREE_UK_FLAG_MMT4D_TYPE_MASK) == IREE_UK_AMD_FLAG_MMT4D_TYPE_F8E4M3FNF8E4M3FNF32 &&
+                           a.ep.out_bytes == 4;
   const int64_t pieces = uk::ceil_div(rm->size1, 8);
   // Rows of tiles a launch: what the buffer holds, and 32-bit numbers of pieces.
   const int64_t panel = (int64_t)p->M0 * (in_place ? pieces * 32 : rm->size1 * 4);
@@ -136,7 +159,8 @@ int launch_epilogue_apart(const iree_uk_mmt4d_params_t* p, const iree_uk_amd_row
       q.out_buffer = a.out;
       q.out_offset = 0;
     }
-    const int st = iree_uk_amd_hip_launch_mmt4d(&q, &r, stream, kernel_mode, kernel_name);
+    const int st = f8_into_f32 ? launch_f8_into_f32(&q, &r, stream, kernel_mode, kernel_name)
+                               : iree_uk_amd_hip_launch_mmt4d(&q, &r, stream, kernel_mode, kernel_name);
     if (st != 0) return st;
     a.z = (const char*)q.out_buffer;
     a.z_pitch = r.stride0 * 4;

@@ -334,3 +334,35 @@ def test_slices_of_a_long_k(gpu, type_, rows, cols, k):
     for i, out in enumerate(("f32", "bf16")):
         names.add(run(lib, type_, rows, cols, k, 16, 16, K0, out, "silu", residual="own", pitch=i, offset=i))
     assert any("kslices" in n for n in names), names
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("K0", [8, 4, 2, 1])
+@pytest.mark.parametrize("residual", [None, "own", "in place"])
+def test_f8_into_f32_keeps_f32_in_any_tile_rows(gpu, K0, residual):
+    """test_f32_matrices_have_sums_in_f32 in tile rows under 16 bytes, from 2^24 multiply-adds on (fewer take the scalar
+    kernel): the same tolerance, and two roundings of the residual's addition."""
+    lib, _ = gpu
+    g = torch.Generator().manual_seed(6)
+    for rows, cols, k, M0 in [(300, 300, 1000, 16), (70, 700, 600, 8), (1000, 1100, 500, 16), (40, 900, 900, 1)]:
+        M1, N1, K1 = -(-rows // M0), -(-cols // 16), -(-k // K0)
+
+        def operand(n, t0, t1):
+            full = torch.zeros(t1 * t0, K1 * K0)
+            full[:n, :k] = 40 * torch.randn(n, k, generator=g)
+            full = full.to(TORCH[F8])
+            return full.view(torch.int8).view(t1, t0, K1, K0).transpose(1, 2).contiguous().cuda(), full[:n].double()
+
+        (lhs, a), (rhs, b) = operand(rows, M0, M1), operand(cols, 16, N1)
+        res = 1000 * torch.randn(rows, cols, generator=g)
+        out = res.cuda() if residual == "in place" else torch.full((rows, cols), 7.0, device="cuda")
+        own = out if residual == "in place" else res.cuda()
+        lib.mmt4d_epilogue_unpack(lhs.data_ptr(), 0, lhs[0].numel(), rhs.data_ptr(), 0, rhs[0].numel(),
+                                  own.data_ptr() if residual else None, 0, cols, out.data_ptr(), 0, cols, rows, cols, None,
+                                  None, None, M1, N1, K1, M0, 16, K0, F8 | uk.MMT4D_ALLOW_GENERIC_FALLBACK_TILE_FUNCTION,
+                                  uk.OUT_TYPE_F32)
+        lib.synchronize()
+        want = a[:, :k] @ b[:, :k].T
+        total = want + (res.double() if residual else 0.0)
+        off = ((out.cpu().double() - total).norm() / want.norm()).item()
+        assert off <= (2 * k ** 0.5 + 2) * U32, (rows, cols, k, M0, off, lib.last_kernel_name())
