@@ -101,11 +101,12 @@ __global__ __launch_bounds__(kThreads) void mmt4d_generic_kernel(Mmt4dArgs a) {
       }
       const float rs = a.row_scale ? a.row_scale[i * M0 + i0] : 1.0f;
       const float cs = a.col_scale ? a.col_scale[j * N0 + j0] : 1.0f;
-      float v = uk::activate(__builtin_fmaf(acc * rs, cs, a.bias ? a.bias[j * N0 + j0] : 0.0f), a.act);
+      const float z = __builtin_fmaf(acc * rs, cs, a.bias ? a.bias[j * N0 + j0] : 0.0f);
       const int64_t ro = (i * M0 + i0) * a.residual_stride + j * N0 + j0;
       auto store = [&](auto type) {
         using F = decltype(type);
         using T = typename F::T;
+        float v = uk::activate<std::is_same<F, uk::F32>::value>(z, a.act);
         if (a.residual) v = F::to_f32(reinterpret_cast<const T*>(a.residual)[ro]) + v;
         reinterpret_cast<T*>(a.out)[o] = F::from_f32(v);
       };

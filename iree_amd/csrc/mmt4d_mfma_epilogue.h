@@ -67,10 +67,19 @@ __device__ __forceinline__ void store_row(const Epilogue& ep, char* out, int row
   }
 }
 
+// The activation of N elements, as close as the matrix's type shows: an f32 one shows the |t|
+// units that a sigmoid may be off (3.7e-6 of the value near t = -80, so 3.7e-7), a 16-bit one,
+// whose half steps are 4.9e-4 and more of it, does not.
+template <int N>
+__device__ __forceinline__ void activate_for(const Epilogue& ep, float (&z)[N]) {
+  if (ep.out_type == IREE_UK_AMD_FLAG_OUT_TYPE_F32) uk::activate_all<true>(z, ep.act);
+  else uk::activate_all(z, ep.act);
+}
+
 // residual + activation(z) of such elements, stored; z has its bias.
 template <int N>
 __device__ __forceinline__ void finish_row(const Epilogue& ep, char* out, int row, int col, int left, float (&z)[N]) {
-  uk::activate_all(z, ep.act);
+  activate_for(ep, z);
   by_out_type(ep, [&](auto type) __attribute__((always_inline)) {
     using F = decltype(type);
     if (ep.residual) {

@@ -1969,7 +1969,7 @@ void mmt4d_mfma_kernel(Args a) {
           const int round = round0 + k;
           float z[8];
           scaled_row((round & (ROUNDS - 1)) * RPI + row0, sm[k], z);
-          uk::activate_all(z, a.ep.act);
+          uk::activate_all<PIECES == 2>(z, a.ep.act);   // (f32 matrices: activate_for)
 #pragma unroll
           for (int h = 0; h < PIECES; ++h) {
             const v4i x = ahead[k][h];

@@ -680,7 +680,7 @@ void mmt4d_thin_kernel(Args a) {
         z[i * 4 + e] = a.col_scale_first ? __builtin_fmaf(v[e] * sn[i][e], sm[i], bias[i][e])
                                          : __builtin_fmaf(v[e] * sm[i], sn[i][e], bias[i][e]);
     }
-    uk::activate_all(z, a.ep.act);
+    activate_for(a.ep, z);
 #pragma unroll
     for (int i = 0; i < OWN; ++i)
 #pragma unroll

@@ -366,3 +366,74 @@ def test_f8_into_f32_keeps_f32_in_any_tile_rows(gpu, K0, residual):
         total = want + (res.double() if residual else 0.0)
         off = ((out.cpu().double() - total).norm() / want.norm()).item()
         assert off <= (2 * k ** 0.5 + 2) * U32, (rows, cols, k, M0, off, lib.last_kernel_name())
+
+
+def epilogue_of_bias(lib, x, rows, k, out, act, N0=16):
+    """The matrix that a product of zeros and a bias of x make: activation(x) in every row."""
+    n = x.numel()
+    M1, N1, K1 = -(-rows // 16), -(-n // N0), -(-k // 16)
+    lhs = torch.zeros(M1, K1, 16, 16, dtype=torch.int8, device="cuda")
+    rhs = torch.zeros(N1, K1, N0, 16, dtype=torch.int8, device="cuda")
+    dt, fo = OUTS[out]
+    y = torch.full((rows, n), 7.0, dtype=dt, device="cuda")
+    lib.mmt4d_epilogue_unpack(lhs.data_ptr(), 0, lhs[0].numel(), rhs.data_ptr(), 0, rhs[0].numel(), None, 0, 0, y.data_ptr(), 0,
+                              n, rows, n, None, None, x.data_ptr(), M1, N1, K1, 16, N0, 16,
+                              S8 | uk.MMT4D_ALLOW_GENERIC_FALLBACK_TILE_FUNCTION, fo | ACTS[act])
+    lib.synchronize()
+    return y
+
+
+def gate_of(lib, x, act):
+    y = torch.empty_like(x)
+    n = x.numel()
+    lib.gate_pack(x.data_ptr(), 0, n, None, 0, 0, y.data_ptr(), 0, n, None, 1, n, 1, n, 1, 1,
+                  uk.IN_TYPE_F32 | uk.OUT_TYPE_F32 | ACTS[act])
+    lib.synchronize()
+    return y.view(1, n)
+
+
+# rows, columns, K: few rows, few columns (operands change places), blocks of 32 to 256 rows, a width that ends inside
+# eight columns, K in slices that another launch adds up.
+BIAS_SIZES = [(1, 4096, 64), (700, 40, 64), (300, 2000, 64), (300, 2003, 64), (2300, 2048, 64), (4096, 4096, 64),
+              (100, 304, 24576)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["silu", "gelu_tanh"])
+def test_sigmoids_into_f32_are_f32(gpu, act):
+    """Into an f32 matrix a sigmoid is as close in its negative tail as near zero. With t the sigmoid's argument, in
+    roundings of 2^-24: e^-t has 2 (the instruction's unit), 1 + e^-t 2, the reciprocal 2, the product with x 1; the
+    remainder -t - hi ln 2 is kept, ln 2 itself being 2.8e-9 off, 0.05 roundings for each unit of t. GELU_TANH's t
+    is four roundings of itself off. What a reciprocal of 2^126 and more would be is lost: |x| 2^-126."""
+    lib, _ = gpu
+
+    def check(y, x, name):
+        v = x.cpu().double().numpy()
+        t = np.abs(v if act == "silu" else v * (1.5957691216 + 0.0713548162726 * v * v))
+        with np.errstate(over="ignore"):
+            want = act64(v, act)
+        slack = np.abs(want) * (8 + (0.05 if act == "silu" else 4.05) * t) * U32 + np.abs(v) * 2.0 ** -126 + 2.0 ** -149
+        off = np.abs(y.cpu().double().numpy() - want) - slack
+        assert off.max() <= 0, (name, act, off.max(), v[off.max(axis=0).argmax()])
+
+    def values(n, seed):
+        g = torch.Generator().manual_seed(seed)
+        x = 4 * torch.randn(n, generator=g)
+        x[::2] = -86 * torch.rand((n + 1) // 2, generator=g) if act == "silu" else -9 * torch.rand((n + 1) // 2, generator=g)
+        return x.cuda()
+
+    x = values(40000, 1)
+    check(gate_of(lib, x, act), x, "gate_pack")
+    names = set()
+    for i, (rows, cols, k) in enumerate(BIAS_SIZES):
+        for mode in MODES:
+            lib.set_kernel_mode(mode)
+            try:
+                x = values(cols, i)
+                check(epilogue_of_bias(lib, x, rows, k, "f32", act), x, (rows, cols, k, lib.last_kernel_name()))
+                names.add(lib.last_kernel_name())
+            finally:
+                lib.set_kernel_mode(uk.KERNEL_MODE_AUTO)
+            if k > 64:
+                break   # (the scalar kernel: no K changes what it does behind its sums)
+    assert len(names) >= 5, names
