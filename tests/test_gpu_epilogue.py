@@ -437,3 +437,37 @@ def test_sigmoids_into_f32_are_f32(gpu, act):
             if k > 64:
                 break   # (the scalar kernel: no K changes what it does behind its sums)
     assert len(names) >= 5, names
+
+
+@pytest.mark.gpu
+def test_gelu_is_its_fit(gpu):
+    """GELU by e^(-s^2/2) t p(t), s = |x|. The constants as they are rounded give the tail s erfc(s / sqrt 2) / 2 to 7.5e-9
+    and to 1.2e-7 s. Roundings of 2^-24 of the tail: 3 of t (its sum, the reciprocal's unit), of which the tail makes 2.8
+    times as much; 3.2 of p, 1 each of three products, 2 of the exponential, 1.25 s^2 of its argument: 17 + 1.25 s^2.
+    One of the result. Over 4096 neighbours those even out but for the units of the reciprocal and of the exponential,
+    which may lean to one side: 8 of the tail, and the fit (one to 1.7e-7 does not pass). For positive x the rounding of
+    x - tail does not even out either: x has no bits below its last, so neighbours whose tails differ by less than
+    that bit (at x = 5 the tail is 1.4e-6, and all of 4096 results are x less the same multiple of 4.8e-7) are all
+    rounded alike, by up to half of it: one rounding of the result more."""
+    lib, _ = gpu
+    windows = 96
+    s = torch.linspace(0.02, 6.5, windows * 4096)
+    for sign in (1.0, -1.0):
+        x = (sign * s).cuda()
+        got = [("gate_pack", gate_of(lib, x, "gelu"))]
+        for lo in range(0, x.numel(), 32 * 4096):
+            part = x[lo:lo + 32 * 4096]
+            got.append((lo, epilogue_of_bias(lib, part, 1, 64, "f32", "gelu")))
+        got = [got[0], ("epilogue", torch.cat([y for _, y in got[1:]], dim=1))]
+        v = x.cpu().double().numpy()
+        a = np.abs(v)
+        want = act64(v, "gelu")
+        tail = 0.5 * a * torch.special.erfc(torch.from_numpy(a * np.sqrt(0.5))).numpy()
+        slack = np.minimum(7.5e-9, 1.2e-7 * a) + tail * (17 + 1.25 * a * a) * U32 + np.abs(want) * U32 + 2.0 ** -125
+        for name, y in got:
+            off = y.cpu().double().numpy()[0] - want
+            assert (np.abs(off) - slack).max() <= 0, (name, sign, (np.abs(off) - slack).max())
+            mean = np.abs(off.reshape(windows, -1).mean(axis=1))
+            limit = 8 * U32 * tail + 4 * slack / 64 + (np.abs(want) * U32 if sign > 0 else 0.0)
+            limit = 7.5e-9 + limit.reshape(windows, -1).mean(axis=1)
+            assert (mean - limit).max() <= 0, (name, sign, mean.max())
