@@ -235,12 +235,15 @@ template <> struct ElemTraits<Elem::kS8Ep> : ElemTraits<Elem::kS8> {};
 template <> struct ElemTraits<Elem::kF16Ep> : ElemTraits<Elem::kF16> {};
 template <> struct ElemTraits<Elem::kBF16Ep> : ElemTraits<Elem::kBF16> {};
 template <> struct ElemTraits<Elem::kF8Ep> : ElemTraits<Elem::kF8> {};
-// 8-bit floats whose sums keep f32: the 8-bit instructions cut the products off at bits of the
-// largest of them (both forms are 1.3e-5 of the root mean square off for normal operands, at any
-// K), which f16's, with the same values, do not (6e-8 at K = 2176). A matrix of 16 bits does not
-// tell the two apart (its own half step is 2.4e-4 and more); one of f32 does. us into bf16 by the 8-bit
-// instructions / into f32 by these: 1 x 28672 x 8192 38.2 / 41.6, 512 x 8192 x 8192 43.6 / 82.3, 4096^3
-// 60.9 / 169 (812 TFLOP/s, bound by f16's rate and the conversions of fragments).
+// 8-bit floats whose sums keep f32: the 8-bit instructions (both forms) add products eight by eight,
+// and of the eight lose what lies 13 binades and more below the largest: 1.5e-5 of the root mean
+// square of the sums for normal operands, at any K, 2^-10 of the sum of magnitudes at most (7
+// products just below 2^-13 of the eighth). f16's, with the same values, do not (6e-8 at K =
+// 2176). An f32 matrix always shows that. A 16-bit one does where an element, or what a residual or a
+// bias leaves of it, is small: 1.5e-5 of the root mean square is the half step of an f16 element of
+// about 5 % of it, of a bf16 one of 0.7 %; such matrices get the faster product all the same. us into
+// bf16 by the 8-bit instructions / into f32 by these: 1 x 28672 x 8192 38.2 / 41.6, 512 x 8192 x 8192 43.6 / 82.3,
+// 4096^3 59.5 / 145 to 169 (812 to 950 TFLOP/s, bound by f16's rate and the conversions of fragments).
 template <> struct ElemTraits<Elem::kF8AsF16Ep> {
   using Acc = v4f;
   using Out = Out32<v4f, float>;

@@ -471,3 +471,49 @@ def test_gelu_is_its_fit(gpu):
             limit = 8 * U32 * tail + 4 * slack / 64 + (np.abs(want) * U32 if sign > 0 else 0.0)
             limit = 7.5e-9 + limit.reshape(windows, -1).mean(axis=1)
             assert (mean - limit).max() <= 0, (name, sign, mean.max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("out", ["f16", "bf16"])
+@pytest.mark.parametrize("spread", ["normal", "binades", "positive binades"])
+def test_f8_into_16_bits_is_off_by_what_its_instructions_lose(gpu, out, spread):
+    """The 8-bit float instructions add products eight by eight and lose what lies 13 binades and more below the largest of
+    the eight: 7 * 2^-13 of it at most, so 2^-10 of the sum of magnitudes; for normal operands 2^-15 of the root mean
+    square at most. Seen behind a residual that cancels the product, so that the matrix's own roundings are small."""
+    lib, _ = gpu
+    g = torch.Generator().manual_seed(8)
+    dt, fo = OUTS[out]
+    half, tiny = HALF[out]
+    for rows, cols, k, M0 in [(1, 64, 512, 1), (16, 300, 4096, 16), (300, 300, 1024, 16), (300, 300, 24608, 16),
+                              (2100, 2100, 512, 16)]:
+        def operand(n, t0):
+            v = torch.exp2(14 * torch.rand(n, k, generator=g) - 6).clamp(max=448)
+            if spread == "normal":
+                v = 40 * torch.randn(n, k, generator=g)
+            elif spread == "binades":
+                v = v * torch.randn(n, k, generator=g).sign()
+            t1 = -(-n // t0)
+            full = torch.zeros(t1 * t0, k)
+            full[:n] = v
+            full = full.to(TORCH[F8])
+            return full.view(torch.int8).view(t1, t0, k // 32, 32).transpose(1, 2).contiguous().cuda(), full[:n].double()
+
+        (lhs, a), (rhs, b) = operand(rows, M0), operand(cols, 16)
+        z, sums = a @ b.T, a.abs() @ b.abs().T
+        scale = 2.0 ** -np.ceil(np.log2(sums.max().item() / 16384))   # (a power of two: exact)
+        z, sums = z * scale, sums * scale
+        res = (-z).to(dt)
+        rs = torch.full((rows,), scale, device="cuda")
+        res_gpu, y = res.cuda(), torch.empty(rows, cols, dtype=dt, device="cuda")
+        lib.mmt4d_epilogue_unpack(lhs.data_ptr(), 0, lhs[0].numel(), rhs.data_ptr(), 0, rhs[0].numel(), res_gpu.data_ptr(), 0,
+                                  cols, y.data_ptr(), 0, cols, rows, cols, rs.data_ptr(), None, None, lhs.shape[0], rhs.shape[0],
+                                  k // 32, M0, 16, 32, F8, fo)
+        lib.synchronize()
+        want = z + res.double()
+        off = (y.cpu().double() - want).abs()
+        # (2^-24 a step of the sum and one for the factor; the matrix's rounding)
+        slack = sums * (2.0 ** -10 + (k / 32 + 2) * U32)
+        assert ((off - (slack + (want.abs() + slack) * half + tiny)).max().item()) <= 0, (rows, cols, k, lib.last_kernel_name())
+        if spread == "normal":
+            rms = lambda t: t.pow(2).mean().sqrt().item()  # noqa: E731
+            assert rms(off) <= 2.0 ** -15 * rms(z) + half * rms(want) + tiny, (rows, cols, k, rms(off) / rms(z))
