@@ -517,3 +517,56 @@ def test_f8_into_16_bits_is_off_by_what_its_instructions_lose(gpu, out, spread):
         if spread == "normal":
             rms = lambda t: t.pow(2).mean().sqrt().item()  # noqa: E731
             assert rms(off) <= 2.0 ** -15 * rms(z) + half * rms(want) + tiny, (rows, cols, k, rms(off) / rms(z))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("residual", [None, "own", "in place"])
+@pytest.mark.parametrize("type_,M0,N0,K0,rows,cols,k", [
+    (S8, 16, 16, 16, 16, 512, 16384), (S8, 32, 16, 8, 40, 264, 512), (BF16, 16, 16, 2, 200, 300, 512),
+    (F16, 16, 16, 8, 520, 776, 320), (F8, 16, 16, 32, 300, 300, 8192), (F8, 1, 16, 32, 1, 1000, 4096),
+    (F8, 16, 16, 8, 100, 120, 256), (F32, 16, 16, 1, 40, 50, 60), (S8, 16, 16, 16, 2050, 2056, 256)])
+def test_every_replay_of_a_captured_epilogue_writes_its_matrix(gpu, type_, M0, N0, K0, rows, cols, k, residual):
+    """The matrix is made unusable before each replay (in place: the residual put back), and compared after it. Small
+    integers throughout: sums are exact, results are roundings of them. Eager calls between the replays."""
+    lib, _ = gpu
+    rng = np.random.default_rng(rows)
+    M1, N1, K1 = -(-rows // M0), -(-cols // N0), -(-k // K0)
+    a, b = rng.integers(-4, 5, (rows, k)).astype(np.float64), rng.integers(-4, 5, (cols, k)).astype(np.float64)
+    lhs, rhs = tiled(a, M0, K0, M1, K1, TORCH[type_]), tiled(b, N0, K0, N1, K1, TORCH[type_])
+    s = torch.cuda.Stream()
+    for out in ("bf16", "f32"):
+        dt, fo = OUTS[out]
+        res = torch.from_numpy(rng.integers(-64, 65, (rows, cols)).astype(np.float32)).to(dt).cuda()
+        want = torch.from_numpy(np.maximum(a @ b.T, 0)).cuda() + (res.double() if residual else 0.0)
+        want = want.to(torch.float32).to(dt)
+        buf = torch.empty(rows, cols, dtype=dt, device="cuda")
+        from_ = None if residual is None else (buf if residual == "in place" else res).data_ptr()
+
+        def call():
+            lib.mmt4d_epilogue_unpack(lhs.data_ptr(), 0, lhs[0].numel(), rhs.data_ptr(), 0, rhs[0].numel(), from_, 0, cols,
+                                      buf.data_ptr(), 0, cols, rows, cols, None, None, None, M1, N1, K1, M0, N0, K0,
+                                      type_ | uk.MMT4D_ALLOW_GENERIC_FALLBACK_TILE_FUNCTION, fo | uk.ACTIVATION_RELU)
+
+        def checked(run_once, what):
+            if residual == "in place":
+                buf.copy_(res)
+            else:
+                buf.fill_(float("nan"))
+            torch.cuda.synchronize()
+            run_once()
+            torch.cuda.synchronize()
+            assert torch.equal(buf, want), (what, out, lib.last_kernel_name(), (buf.double() - want.double()).abs().max().item())
+
+        torch.cuda.synchronize()
+        lib.set_stream(s.cuda_stream)
+        lib.set_pointer_mode(uk.POINTER_MODE_DEVICE)
+        try:
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=s):
+                call()
+            for i in range(3):
+                checked(g.replay, "replay %d" % i)
+                checked(call, "eager %d" % i)
+        finally:
+            lib.set_stream(None)
+            lib.set_pointer_mode(uk.POINTER_MODE_AUTO)
