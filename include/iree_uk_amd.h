@@ -762,7 +762,8 @@ enum {
   /* Activation:  NONE  x;  RELU  x < 0 ? 0 : x;  SILU  x / (1 + e^-x);
    *   GELU       x/2 * (1 + erf(x / sqrt 2));
    *   GELU_TANH  x/2 * (1 + tanh(sqrt(2/pi) * (x + 0.044715 x^3))).
-   * The lowest numbers give zero, -infinity zero (RELU, GELU) or NaN. */
+   * The lowest numbers give zero, -infinity zero (RELU, GELU) or NaN. A sigmoid
+   * below 2^-126 (SILU below -87) counts as zero. */
   IREE_UK_AMD_FLAG_ACTIVATION_MASK = 0xF00,
   IREE_UK_AMD_FLAG_ACTIVATION_NONE = 0x000,
   IREE_UK_AMD_FLAG_ACTIVATION_RELU = 0x100,
@@ -787,9 +788,13 @@ enum {
  *                        row_scale[row] = max|y| / 127 (S8), / 448 (F8E4M3FN):
  *                        the row scales of iree_uk_amd_mmt4d_dequant_unpack
  *                        and iree_uk_amd_mmt4d_epilogue_unpack.
- * Rows with no 8-bit form: where max|y| is zero (or below 2^-100, whose scale
- * has no usable inverse) the scale is 0 and the row zeros; where the row holds
- * a NaN or an infinity, or its sum of squares exceeds f32, the scale is NaN and
+ * h * weight is formed before the division, in f32: where it is beyond f32, y is
+ * infinite. Rows that have no norm, because they hold a NaN or an infinity or
+ * because their sum of squares exceeds f32, are NaN in the in type; the tiles
+ * around them are zeros as around any other.
+ * Rows with no 8-bit form: where max|y| is zero (or below 2^-100, or
+ * max|h * weight| below 2^-110, whose scales have no usable inverse) the scale
+ * is 0 and the row zeros; where y holds a NaN or an infinity the scale is NaN and
  * the row zeros, so that every result that the row enters is NaN.
  *
  * in, residual and sum have the in type, rows of contiguous columns and
@@ -898,8 +903,9 @@ IREE_UK_AMD_EXPORT void iree_uk_amd_gate_pack_p(
  * elements in common. Operand arguments, tile sizes and `flags` are those of
  * iree_uk_mmt4d for a type with a 32-bit accumulator, without ACCUMULATE;
  * `epilogue_flags` is out type | activation; out_stride0 >= out_size1 (where
- * there is more than one row), residual_stride0 >= 0. K == 0 is a product of zeros. out_size0 <= M*M0 and out_size1 <=
- * N*N0; elements between and behind the rows stay as they are.
+ * there is more than one row), residual_stride0 >= 0. K == 0 is a product of
+ * zeros. out_size0 <= M*M0 and out_size1 <= N*N0; elements between and behind
+ * the rows stay as they are.
  *
  * Sums are f32 (s32 for integers). f8 into f16 and bf16 multiplies on the 8-bit
  * float instructions, which add products eight by eight and lose what lies 13
@@ -911,14 +917,18 @@ IREE_UK_AMD_EXPORT void iree_uk_amd_gate_pack_p(
  * f8 into f32 multiplies the same values as f16 instead, at half the rate and
  * less, without that error.
  *
- * One launch, and no memory beyond the operands but a workspace like iree_uk_mmt4d's
- * for sums in parts of K (with a launch or two more; up to 75 MB), for s8 (tile rows of 8 bytes and more), f16, bf16 and f8 (16
- * bytes and more, what iree_uk_query_tile_sizes_2d answers with) and s8 x s4.
- * Other types and tile rows run as a product into f32 and an epilogue of its
- * own, in place for an f32 matrix, else from a buffer that the library keeps per
- * thread and stream (64 MB, or one row of tiles; workspace_bytes and
- * release_workspaces count it). On a stream that is being captured there is no
- * such buffer and they take the scalar kernel: graphs want 16-byte tile rows. */
+ * One launch, and no memory beyond the operands but a workspace like
+ * iree_uk_mmt4d's for sums in parts of K (with a launch or two more; up to 64
+ * MB; none on a stream that is being captured, where K stays whole), for s8
+ * (tile rows of 8 bytes and more), f16, bf16 and f8 (16 bytes and more, what
+ * iree_uk_query_tile_sizes_2d answers with) and s8 x s4 (16 elements and more;
+ * from 512 rows on the weights are widened first, as by iree_uk_mmt4d). Other
+ * types and tile rows run as a product into f32 and an epilogue of its own: in
+ * place for an f32 matrix whose residual is another one, else from a buffer
+ * that the library keeps per thread and stream (64 MB, or one row of tiles;
+ * workspace_bytes and release_workspaces count it). On a stream that is being
+ * captured there is no such buffer, nor one for regrouped tiles, and calls that
+ * need one take the scalar kernel: graphs want 16-byte tile rows. */
 typedef struct iree_uk_amd_mmt4d_epilogue_unpack_params_t {
   const void* lhs_buffer;
   iree_uk_index_t lhs_offset;

@@ -525,3 +525,29 @@ def test_norm_padding_is_zero_whatever_the_rows_hold(gpu, tin, cols):
         assert np.isnan(got[1, :cols]).all() if eps == 0 else not got[1].any(), name
         keep = [0, 5]
         check_rows(y[keep], slack[keep], tin, tin, tiles[:1][:, :, keep, :], None, 2, cols, name)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cols", [70, 40000])
+def test_norm_forms_the_weighted_row_before_it_divides(gpu, cols):
+    """Weights that take h beyond f32, or below what has an inverse: infinities and scales of NaN and 0, as the header says,
+    where the quotient times the weight would be a number. Squares that f32 does not hold: NaN."""
+    lib, _ = gpu
+    K1 = -(-cols // 16)
+    for h, w, value, scale in [(1e15, 1e30, math.inf, math.nan), (2.0 ** -60, 2.0 ** -55, 2.0 ** -55, 0.0), (1e20, 1.0, math.nan, math.nan),
+                               (2.0 ** -60, 2.0 ** -45, 2.0 ** -45, 2.0 ** -45 / 127)]:
+        x = torch.full((2, cols), h, device="cuda")
+        weight = torch.full((cols,), w, device="cuda")
+        y = torch.full((2, K1, 1, 16), 7.0, device="cuda")
+        q = torch.full((2, K1, 1, 16), 7, dtype=torch.int8, device="cuda")
+        s = torch.full((2,), 7.0, device="cuda")
+        for out, fo in ((y, uk.OUT_TYPE_F32), (q, uk.OUT_TYPE_S8)):
+            lib.rmsnorm_pack(x.data_ptr(), 0, cols, None, 0, 0, None, 0, 0, weight.data_ptr(), 0.0, out.data_ptr(), 0,
+                             out.stride(0), s.data_ptr(), 2, cols, 2, K1, 1, 16, uk.IN_TYPE_F32 | fo)
+        lib.synchronize()
+        # (the sum of squares is off by cols / 64 roundings and the scale by a few)
+        same = dict(rtol=(cols / 64 + 32) * U32, atol=0.0, equal_nan=True)
+        assert np.allclose(y.cpu().numpy().reshape(2, -1)[:, :cols], value, **same), (h, w)
+        assert np.allclose(s.cpu().numpy(), scale, **same), (h, w, s)
+        assert bool((q.view(2, -1)[:, :cols] == (127 if scale > 0 else 0)).all()) and not q.view(2, -1)[:, cols:].any(), (h, w)
+        assert not y.view(2, -1)[:, cols:].any(), (h, w)
