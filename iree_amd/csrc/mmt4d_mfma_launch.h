@@ -971,7 +971,8 @@ int slices_that_pay(const Problem& p, int64_t rows, int64_t cols, bool long_k) {
   // In front of an epilogue blocks that fill more than half of the units have slices in several
   // rounds, if K ends inside a step or is long (us in 64x64 blocks / here: s8 1500 x 1500 x 28672
   // 128.7 / 93.7, 700 x 3000 x 25695 149.3 / 92.6, bf16 1600 x 1600 x 12288 105.6 / 85.1, f16 1366 x 1614 x
-  // 7236 73.9 / 61.0); five at most, whose sums take 63 MB of the workspace.
+  // 7236 73.9 / 61.0); five at most. (The sums and those of the end of K take 63 MB of the workspace at
+  // most: five slices pay up to 153 blocks of 256 units, four up to 191.)
   if (has_epilogue<E>() && (long_k || rest) && slices < 2) {
     for (int64_t n = 2; n <= std::min<int64_t>(most, 5); ++n)
       if (slices < 2 || cost(n) < cost(slices)) slices = n;

@@ -570,3 +570,19 @@ def test_every_replay_of_a_captured_epilogue_writes_its_matrix(gpu, type_, M0, N
         finally:
             lib.set_stream(None)
             lib.set_pointer_mode(uk.POINTER_MODE_AUTO)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,cols", [(1792, 1664), (1920, 1280)])
+def test_slices_keep_the_memory_that_the_header_names(gpu, rows, cols):
+    """182 and 150 blocks of 64 KB with K in slices of whole steps, and its end as one more: 64 MB of sums, and the workspace's
+    counters. (At 24 KB of K the costs are 115 us for four slices of 182 blocks, 96 for three of 150, where five, from
+    42 KB on, would keep as much: 60 MB.)"""
+    lib, _ = gpu
+    lib.release_workspaces()
+    name = run(lib, S8, rows, cols, 24603, 16, 16, 16, "bf16", "none", residual="own")
+    assert "kslices" in name and lib.last_k_slices() >= 3, (name, lib.last_k_slices())
+    kept = lib.workspace_bytes()
+    assert 0 < kept <= (64 << 20) + (64 << 10), kept
+    lib.release_workspaces()
+    assert lib.workspace_bytes() == 0
