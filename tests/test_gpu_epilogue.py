@@ -586,3 +586,67 @@ def test_slices_keep_the_memory_that_the_header_names(gpu, rows, cols):
     assert 0 < kept <= (64 << 20) + (64 << 10), kept
     lib.release_workspaces()
     assert lib.workspace_bytes() == 0
+
+
+def exact_epilogue(lib, type_, rows, cols, k, M0, N0, K0, out, *, residual, panels=(0, 0), on="cuda", seed=0):
+    """A call whose results are exact: small integers, row scales of powers of two, RELU. `residual`: None, "own", "in place"
+    or "one row" (a stride of 0). `panels`: tiles beyond those that the matrix needs, which hold what must not matter."""
+    rng = np.random.default_rng(seed)
+    M1, N1, K1 = -(-rows // M0) + panels[0], -(-cols // N0) + panels[1], -(-k // K0)
+    a, b = rng.integers(-4, 5, (rows, k)).astype(np.float64), rng.integers(-4, 5, (cols, k)).astype(np.float64)
+    lhs, rhs = tiled(a, M0, K0, M1, K1, TORCH[type_]).to(on), tiled(b, N0, K0, N1, K1, TORCH[type_]).to(on)
+    dt, fo = OUTS[out]
+    rs = torch.exp2(torch.from_numpy(rng.integers(-2, 3, rows)).float())
+    n_res = 1 if residual == "one row" else rows
+    res = torch.from_numpy(rng.integers(-64, 65, (n_res, cols)).astype(np.float32)).to(dt)
+    want = torch.from_numpy(np.maximum(a @ b.T, 0)) * rs.double()[:, None] + (res.double() if residual else 0.0)
+    want = want.float().to(dt)
+    buf = torch.full((rows + 1, cols + 3), 7.0, dtype=dt)
+    if residual == "in place":
+        buf[:rows, :cols] = res
+    before = buf.clone()
+    buf, rs_on, res_on = buf.to(on), rs.to(on), res.to(on)
+    from_, stride = {None: (None, 0), "own": (res_on, cols), "one row": (res_on, 0), "in place": (buf, cols + 3)}[residual]
+    lib.mmt4d_epilogue_unpack(lhs.data_ptr(), 0, lhs[0].numel(), rhs.data_ptr(), 0, rhs[0].numel(),
+                              from_.data_ptr() if from_ is not None else None, 0, stride, buf.data_ptr(), 0, cols + 3, rows,
+                              cols, rs_on.data_ptr(), None, None, M1, N1, K1, M0, N0, K0,
+                              type_ | uk.MMT4D_ALLOW_GENERIC_FALLBACK_TILE_FUNCTION, fo | uk.ACTIVATION_RELU)
+    name = (type_, rows, cols, k, M0, N0, K0, out, residual, panels, on, lib.last_kernel_name())
+    lib.synchronize()
+    got = buf.cpu()
+    assert torch.equal(got[:rows, :cols], want), name
+    got[:rows, :cols] = before[:rows, :cols]
+    assert torch.equal(got, before), name
+    return name[-1]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type_,M0,N0,K0", [(F32, 16, 16, 4), (F32, 1, 16, 1), (BF16, 16, 16, 2), (F8, 16, 16, 8)])
+@pytest.mark.parametrize("residual", [None, "own", "in place", "one row"])
+def test_a_product_apart_in_several_rounds_of_rows(gpu, type_, M0, N0, K0, residual):
+    """Products of more than 64 MB of f32 in front of an epilogue of their own: rounds of rows, each with its scales and
+    its rows of the residual."""
+    lib, _ = gpu
+    for out in ("f32", "bf16"):
+        exact_epilogue(lib, type_, 4501, 4099, 24, M0, N0, K0, out, residual=residual)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type_,M0,N0,K0", [(S8, 16, 16, 16), (S8, 1, 16, 16), (S8, 32, 16, 8), (F8, 16, 16, 32), (F8, 16, 16, 4),
+                                            (BF16, 16, 16, 8), (F16, 24, 12, 8), (F32, 16, 16, 4)])
+def test_tiles_beyond_the_matrix_and_a_residual_of_one_row(gpu, type_, M0, N0, K0):
+    """More tiles than the matrix has rows and columns for, from one row to several rounds of blocks and K in slices; a
+    residual whose rows are all the same one."""
+    lib, _ = gpu
+    for i, (rows, cols, k) in enumerate([(1, 300, 256), (3, 70, 1030), (40, 33, 512), (300, 500, 200), (700, 1500, 320),
+                                         (130, 300, 24703), (2050, 2060, 96)]):
+        for out, residual in (("bf16", "one row"), ("f32", "in place"), ("f32", "one row")):
+            exact_epilogue(lib, type_, rows, cols, k, M0, N0, K0, out, residual=residual, panels=(i % 3, (i + 1) % 4), seed=i)
+
+
+@pytest.mark.gpu
+def test_epilogue_on_host_memory_with_a_residual_of_one_row(gpu):
+    lib, _ = gpu
+    for out in ("f32", "bf16"):
+        for residual in ("one row", "in place", "own", None):
+            exact_epilogue(lib, S8, 37, 50, 96, 16, 16, 16, out, residual=residual, panels=(1, 1), on="cpu")

@@ -551,3 +551,33 @@ def test_norm_forms_the_weighted_row_before_it_divides(gpu, cols):
         assert np.allclose(s.cpu().numpy(), scale, **same), (h, w, s)
         assert bool((q.view(2, -1)[:, :cols] == (127 if scale > 0 else 0)).all()) and not q.view(2, -1)[:, cols:].any(), (h, w)
         assert not y.view(2, -1)[:, cols:].any(), (h, w)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cols", [200, 40000])
+@pytest.mark.parametrize("on", ["cuda", "cpu"])
+def test_inputs_of_one_row_for_all(gpu, cols, on):
+    """A stride of 0: the same row of x beside every row of the residual, the same gate beside every row of up."""
+    lib, _ = gpu
+    g = torch.Generator().manual_seed(cols)
+    one, many = torch.randn(1, cols, generator=g).to(on), torch.randn(5, cols, generator=g).to(on)
+    all_ = one.expand(5, cols).contiguous()
+    K1 = -(-cols // 16)
+
+    def run(first, second, strides, norm):
+        q = torch.full((1, K1, 16, 16), 7, dtype=torch.int8, device=on)
+        s, total = torch.full((5,), 7.0, device=on), torch.full((5, cols), 7.0, device=on)
+        args = (first.data_ptr(), 0, strides[0], second.data_ptr(), 0, strides[1])
+        into = (q.data_ptr(), 0, q.numel(), s.data_ptr(), 5, cols, 1, K1, 16, 16, uk.IN_TYPE_F32 | uk.OUT_TYPE_S8)
+        if norm:
+            lib.rmsnorm_pack(*args, total.data_ptr(), 0, cols, None, 1e-5, *into)
+        else:
+            lib.gate_pack(*args, *into[:-1], into[-1] | uk.ACTIVATION_SILU)
+        lib.synchronize()
+        return q, s, total
+
+    for norm in (True, False):
+        for wide, narrow in ((run(all_, many, (cols, cols), norm), run(one, many, (0, cols), norm)),
+                             (run(many, all_, (cols, cols), norm), run(many, one, (cols, 0), norm))):
+            assert all(torch.equal(a, b) for a, b in zip(wide, narrow)), (norm, cols, on)
+            assert wide[0].any() and (wide[1] > 0).all()
